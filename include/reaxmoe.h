@@ -19,6 +19,8 @@
  *   - the decision forward's element-wise steps around the MoE block (Gemma4DecoderLayer.forward, gemma4.py:696-771:
  *     RMSNorm + bf16 adds, q/k/v norms + RoPE, GELU-tanh * up)  -> reaxmoe_rmsnorm, reaxmoe_qkv_norm_rope,
  *                                                                    reaxmoe_gelu_tanh_mul
+ *   - its attention over packed prompts (Gemma4Attention.forward, gemma4.py:505-539)
+ *                                                                 -> reaxmoe_attention
  *   - get_cutlass_moe_mm_data / blink _fplan (champions/uid240/opt/blink/blink_moe.py:271-299)
  *                                                                                 -> reaxmoe_plan
  *   - scaled_fp4_experts_quant of the m rows + _tscatter (blink_moe.py:301-323, :402-421)
@@ -164,6 +166,46 @@ int reaxmoe_qkv_norm_rope(const void* qkv, const void* q_weight, const void* k_w
                           int32_t kv_heads, int32_t head_dim, void* q, void* k, void* v, void* stream);
 /* gate_up [rows, 2 inter] -> out [rows, inter] = bf16(bf16(gelu_tanh(gate)) * up) (GeluAndMul native form). */
 int reaxmoe_gelu_tanh_mul(const void* gate_up, int64_t rows, int32_t inter, void* out, void* stream);
+
+/* ---- Attention over packed sequences (Gemma4Attention.forward's attention, gemma4.py:505-539, and the same for a batch
+ * that continues one shared prefix). Sequence b has query rows [cu_q[b], cu_q[b + 1]) of q and keys [cu_k[b], cu_k[b + 1])
+ * of k / v, behind `prefix` keys of prefix_k / prefix_v that every sequence sees first and that are stored once. With m
+ * query rows and n own keys, row i stands at position t = prefix + n - m + i of the virtual key axis (prefix, then own
+ * keys) and sees keys j of it with
+ *     j <= t (causal) or every j;   j > t - window when window > 0.
+ * out[row] = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max), s_j = scale * q . k_j over the keys seen (bf16 / fp16
+ * products, fp32 sums; the weights exp(s_j - max) enter the second product rounded to the operands' type), and lse[row] =
+ * max + log(sum). A row that sees no key gets out 0 and lse -inf. Keys that a row does not see do not change it, whatever
+ * their values (infinities and NaN included). Query head h reads KV head h / (q_heads / kv_heads). Rows of q at and behind
+ * cu_q[seqs] are not written. Inference only: there is no backward. */
+enum { REAXMOE_BF16 = 0, REAXMOE_FP16 = 1 };
+
+typedef struct reaxmoe_attention_args {
+  const void* q;              /* [q_tokens, q_heads, head_dim] */
+  const void* k;              /* [k_tokens, kv_heads, head_dim]; may be NULL when k_tokens == 0 (v too) */
+  const void* v;
+  const void* prefix_k;       /* [prefix, kv_heads, head_dim]; NULL when prefix == 0 */
+  const void* prefix_v;
+  const int32_t* cu_q;        /* [seqs + 1], non-decreasing from 0 (device) */
+  const int32_t* cu_k;        /* [seqs + 1] */
+  void* out;                  /* [q_tokens, q_heads, head_dim] in the type of q; overlaps no input */
+  float* lse;                 /* [q_tokens, q_heads] or NULL */
+  int32_t* status;            /* device word or NULL: receives REAXMOE_ERR_DEVICE_TIMEOUT if a bounded wait expires */
+  /* strides in elements, between tokens and between heads (the last dimension is contiguous); multiples of 8 */
+  int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+  int64_t prefix_k_stride, prefix_k_head_stride, prefix_v_stride, prefix_v_head_stride, out_stride, out_head_stride;
+  int64_t q_tokens, k_tokens, prefix;   /* prefix + k_tokens < 2^31 - 2^16, q_tokens * q_heads / kv_heads < 2^31 - 2^16 */
+  int32_t seqs, q_heads, kv_heads, head_dim;   /* q_heads a multiple of kv_heads; head_dim 64, 128 or 256 */
+  int32_t dtype;              /* REAXMOE_BF16 or REAXMOE_FP16 */
+  int32_t causal;             /* 0 or 1 */
+  int32_t window;             /* 0: none; else >= 1, with causal */
+  float scale;                /* > 0 */
+} reaxmoe_attention_args;
+
+/* Bytes of workspace reaxmoe_attention needs for these sizes (at least 256; 0 on bad sizes). It depends on the sizes alone,
+ * not on the cumulative lengths. */
+size_t reaxmoe_attention_workspace_size(const reaxmoe_attention_args* args);
+int reaxmoe_attention(const reaxmoe_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Routing data (get_cutlass_moe_mm_data; blink_moe.py:271-299). Writes, inside the workspace, the per-expert
  * counts, expert_offsets[E+1], blockscale_offsets[E+1] and GEMM tile tables, and copies them out to the

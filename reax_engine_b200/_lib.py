@@ -23,6 +23,9 @@ ERR_UNSUPPORTED = 9
 ACT_SILU = 0
 ACT_GELU_TANH = 1
 
+BF16 = 0
+FP16 = 1
+
 ERROR_NAMES = {
     ERR_BAD_SHAPE: "BAD_SHAPE", ERR_MISALIGNED: "MISALIGNED", ERR_TOO_MANY_EXPERTS: "TOO_MANY_EXPERTS",
     ERR_DEVICE_TIMEOUT: "DEVICE_TIMEOUT", ERR_WORKSPACE: "WORKSPACE", ERR_CUDA: "CUDA", ERR_NULL: "NULL",
@@ -47,6 +50,16 @@ class ForwardArgs(ctypes.Structure):
         "topk_weights", "topk_ids", "output")]
 
 
+class AttentionArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "prefix_k", "prefix_v", "cu_q", "cu_k", "out", "lse", "status")]
+                + [(n, ctypes.c_int64) for n in (
+                    "q_stride", "q_head_stride", "k_stride", "k_head_stride", "v_stride", "v_head_stride",
+                    "prefix_k_stride", "prefix_k_head_stride", "prefix_v_stride", "prefix_v_head_stride", "out_stride",
+                    "out_head_stride", "q_tokens", "k_tokens", "prefix")]
+                + [(n, ctypes.c_int32) for n in ("seqs", "q_heads", "kv_heads", "head_dim", "dtype", "causal", "window")]
+                + [("scale", ctypes.c_float)])
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -69,6 +82,8 @@ SIGNATURES = {
                                              _P, _P, _P, _P]),
     "reaxmoe_forward_prequant": (ctypes.c_int, [ctypes.POINTER(ForwardArgs), _P, ctypes.c_float, _P, ctypes.c_size_t,
                                                 _P]),
+    "reaxmoe_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttentionArgs)]),
+    "reaxmoe_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _P, ctypes.c_size_t, _P]),
     "reaxmoe_plan": (ctypes.c_int, [_PP, _P, _P, ctypes.c_size_t, _P, _P, _P, _P, _P]),
     "reaxmoe_permute_quant": (ctypes.c_int, [_PP, _P, _P, _P, _P, ctypes.c_size_t, _P, _P, _P, _P]),
     "reaxmoe_gemm_w13": (ctypes.c_int, [_PP, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P, _P, _P]),

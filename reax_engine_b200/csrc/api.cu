@@ -442,6 +442,73 @@ int reaxmoe_gelu_tanh_mul(const void* gate_up, int64_t rows, int32_t inter, void
   return cuda_check("gelu_tanh_mul");
 }
 
+static int check_attention_sizes(const reaxmoe_attention_args* a) {
+  if (a == nullptr) return fail(REAXMOE_ERR_NULL, "attention: args is NULL");
+  constexpr int64_t kMax = 0x7FFFFFFFll - 65536;   // row and key numbers, and tile ends past them, fit an int
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: head_dim=%d (64, 128 or 256)", a->head_dim);
+  if (a->q_heads < 1 || a->kv_heads < 1 || a->kv_heads > 65535 || a->q_heads % a->kv_heads != 0)
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: q_heads=%d must be a multiple of kv_heads=%d (at most 65535)", a->q_heads,
+                a->kv_heads);
+  if (a->seqs < 0 || a->q_tokens < 0 || a->k_tokens < 0 || a->prefix < 0 || a->q_tokens > kMax || a->k_tokens > kMax ||
+      a->prefix > kMax || a->prefix + a->k_tokens > kMax || a->q_tokens * (a->q_heads / a->kv_heads) > kMax)
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: seqs=%d q_tokens=%lld k_tokens=%lld prefix=%lld out of range", a->seqs,
+                (long long)a->q_tokens, (long long)a->k_tokens, (long long)a->prefix);
+  if (a->dtype != REAXMOE_BF16 && a->dtype != REAXMOE_FP16)
+    return fail(REAXMOE_ERR_UNSUPPORTED, "attention: dtype=%d (bf16 or fp16)", a->dtype);
+  if ((a->causal != 0 && a->causal != 1) || a->window < 0 || (a->window > 0 && !a->causal))
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: causal=%d window=%d (a window needs causal)", a->causal, a->window);
+  if (!(a->scale > 0.0f) || a->scale > 3.0e38f)
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: scale must be positive and finite");
+  return 0;
+}
+
+// strides of a [tokens, heads, head_dim] tensor: 16-byte rows that do not overlap, within the tensor map's 2^40 bytes
+static bool bad_strides(int64_t token, int64_t head, int heads, int64_t tokens, int d) {
+  if ((token | head) & 7) return true;
+  if (token < 0 || head < 0 || token >= (int64_t)1 << 38 || head >= (int64_t)1 << 38) return true;
+  if (heads > 1 && head < d) return true;
+  return tokens > 1 && token < d;
+}
+
+size_t reaxmoe_attention_workspace_size(const reaxmoe_attention_args* args) {
+  if (check_attention_sizes(args)) return 0;
+  return attention_workspace(*args, num_sms());
+}
+
+int reaxmoe_attention(const reaxmoe_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check_attention_sizes(args)) return rc;
+  const reaxmoe_attention_args& a = *args;
+  if (a.q_tokens == 0 || a.seqs == 0) return 0;
+  if (!a.q || !a.cu_q || !a.cu_k || !a.out || (a.k_tokens > 0 && (!a.k || !a.v)) ||
+      (a.prefix > 0 && (!a.prefix_k || !a.prefix_v)))
+    return fail(REAXMOE_ERR_NULL, "attention: NULL pointer");
+  if (!aligned16(a.q) || !aligned16(a.out) || (a.k_tokens > 0 && (!aligned16(a.k) || !aligned16(a.v))) ||
+      (a.prefix > 0 && (!aligned16(a.prefix_k) || !aligned16(a.prefix_v))))
+    return fail(REAXMOE_ERR_MISALIGNED, "attention: tensors must be 16-byte aligned");
+  const int d = a.head_dim;
+  if (bad_strides(a.q_stride, a.q_head_stride, a.q_heads, a.q_tokens, d) ||
+      bad_strides(a.out_stride, a.out_head_stride, a.q_heads, a.q_tokens, d) ||
+      (a.k_tokens > 0 && (bad_strides(a.k_stride, a.k_head_stride, a.kv_heads, a.k_tokens, d) ||
+                          bad_strides(a.v_stride, a.v_head_stride, a.kv_heads, a.k_tokens, d))) ||
+      (a.prefix > 0 && (bad_strides(a.prefix_k_stride, a.prefix_k_head_stride, a.kv_heads, a.prefix, d) ||
+                        bad_strides(a.prefix_v_stride, a.prefix_v_head_stride, a.kv_heads, a.prefix, d))))
+    return fail(REAXMOE_ERR_MISALIGNED, "attention: strides must be multiples of 8 elements and rows must not overlap");
+  AttentionLaunch l;
+  memset(&l, 0, sizeof(l));
+  l.a = a;
+  l.num_sms = num_sms();
+  l.timeout_ns = device_timeout_ns();
+  l.workspace = workspace;
+  const size_t need = attention_workspace(a, l.num_sms);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(REAXMOE_ERR_WORKSPACE, "attention: workspace %zu bytes < required %zu", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(REAXMOE_ERR_MISALIGNED, "attention: workspace not 16-byte aligned");
+  const int rc = launch_attention(l, static_cast<cudaStream_t>(stream));
+  if (rc) return fail(rc, "attention launch failed: %s", cudaGetErrorString(cudaPeekAtLastError()));
+  return cuda_check("attention");
+}
+
 int reaxmoe_plan(const reaxmoe_problem* p, const int32_t* topk_ids, void* workspace, size_t workspace_bytes,
                  int32_t* expert_offsets, int32_t* blockscale_offsets, int32_t* problem_sizes1,
                  int32_t* problem_sizes2, void* stream) {

@@ -147,6 +147,16 @@ struct RouterLaunch {
 };
 int launch_router_topk(const RouterLaunch& r, cudaStream_t s);
 
+// Packed-sequence attention (attention.cu).
+struct AttentionLaunch {
+  reaxmoe_attention_args a;
+  void* workspace;
+  unsigned long long timeout_ns;
+  int num_sms;
+};
+size_t attention_workspace(const reaxmoe_attention_args& a, int num_sms);
+int launch_attention(const AttentionLaunch& l, cudaStream_t s);
+
 // decision_ops.cu: the decision forward's fused element-wise steps
 int launch_rmsnorm(const void* a, const void* b, const void* w, const void* res, float eps, int64_t rows, int cols,
                    void* out, cudaStream_t s);
