@@ -17,23 +17,27 @@ struct RowKeys {
   int k_lo, k_hi;   // keys of the packed k / v seen (row numbers of the packed tensors)
 };
 
-// Keys that query token t sees. t < min(cu_q[seqs], q_tokens); the cumulative lengths are cut to the tensors, so that no
-// value of theirs makes a later access leave them.
-__device__ __forceinline__ RowKeys row_keys(const reaxmoe_attention_args& a, int t) {
-  int b0 = 0, b1 = a.seqs;                       // the last b with cu_q[b] <= t (sequences of no rows are passed over)
+// the last b with cu_q[b] <= t (sequences of no rows are passed over); t < cu_q[seqs]
+__device__ __forceinline__ int sequence_of(const reaxmoe_attention_args& a, int t) {
+  int b0 = 0, b1 = a.seqs;
   while (b1 - b0 > 1) {
     const int mid = (b0 + b1) >> 1;
     if (__ldg(a.cu_q + mid) <= t) b0 = mid; else b1 = mid;
   }
-  const int q0 = __ldg(a.cu_q + b0), q1 = __ldg(a.cu_q + b0 + 1);
+  return b0;
+}
+
+// Keys that query token t of sequence b sees. The cumulative lengths are cut to the tensors, so that no value of theirs makes
+// a later access leave them.
+__device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
   const int kt = (int)a.k_tokens, P = (int)a.prefix;
-  const int ks = min(max(__ldg(a.cu_k + b0), 0), kt);
-  const int n = min(max(__ldg(a.cu_k + b0 + 1), ks), kt) - ks;
-  const int64_t pos = (int64_t)P + n - ((int64_t)q1 - t);          // prefix + n - m + (t - q0)
-  (void)q0;
-  int64_t hi = a.causal ? pos + 1 : (int64_t)P + n;
+  const int ks = min(max(__ldg(a.cu_k + b), 0), kt);
+  const int n = min(max(__ldg(a.cu_k + b + 1), ks), kt) - ks;
+  const int64_t pos = (int64_t)P + n - ((int64_t)__ldg(a.cu_q + b + 1) - t);    // prefix + n - m + i
+  const int64_t all = (int64_t)P + n;
+  int64_t hi = a.causal ? pos + 1 : all;
   int64_t lo = a.window > 0 ? pos - a.window + 1 : 0;
-  hi = hi < 0 ? 0 : (hi > (int64_t)P + n ? (int64_t)P + n : hi);
+  hi = hi < 0 ? 0 : (hi > all ? all : hi);
   lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
   RowKeys r;
   r.p_lo = (int)(lo < P ? lo : P);
@@ -41,6 +45,9 @@ __device__ __forceinline__ RowKeys row_keys(const reaxmoe_attention_args& a, int
   r.k_lo = ks + (int)(lo > P ? lo - P : 0);
   r.k_hi = ks + (int)(hi > P ? hi - P : 0);
   return r;
+}
+__device__ __forceinline__ RowKeys row_keys(const reaxmoe_attention_args& a, int t) {
+  return row_keys_of(a, sequence_of(a, t), t);
 }
 
 template <bool BF>
