@@ -18,13 +18,13 @@
 //   S = Q K^T          [256 x 128], Q and K from shared memory (128-byte swizzle, K-major);
 //   P = exp2(c S - c m) by 8 warps per CTA, packed to 16 bits over the first half of S's own TMEM columns;
 //   O += P V           [256 x D], P from TMEM, V from shared memory as it lies in memory (MN-major).
-// S is double-buffered (2 x 128 columns) beside O (D columns): the tensor core multiplies S(j + 1) while the softmax of tile j
-// runs, and the next item's first two S while this item's O is written out.
+// S has 2 buffers of 128 columns beside O (D columns) for D = 256, 3 for D <= 128: the tensor core multiplies S(j + 1) (and
+// S(j + 2)) while the softmax of tile j runs, and the next item's first S while this item's O is written out.
 //
-//   warps 0..7    softmax: TMEM lane quarter w % 4 (thread = row), column half w / 4; the halves of a row meet in shared memory
+//   warps 0..7    softmax: TMEM lane quarter w % 4 (thread = row), column half w / 4; the halves of a row exchange maxima
 //   warp 8        K / V producer: ring of slots, alternately half a K tile (64 keys x D) and half a V tile (128 keys x D / 2)
 //   warp 9        allocates TMEM; in the leader CTA one thread issues all MMAs of the pair
-//   warps 10..13  loader: takes the next item, works out its key ranges, copies its Q rows
+//   warps 10, 11  loader: takes the next item, works out its key ranges, copies its Q rows
 // Items (row tile, KV head, part of the keys) are taken in order, the first by pair number, further ones from a counter.
 // With few rows an item's keys are split over several pairs, which leave partial sums that combine_kernel joins.
 // All waits are bounded (globaltimer); a timeout records REAXMOE_ERR_DEVICE_TIMEOUT and the CTA winds down.
@@ -40,18 +40,19 @@ namespace attn {
 constexpr int ROWS = 128;                 // query rows per CTA
 constexpr int KT = 128;                   // keys per tile
 constexpr int SM_WARPS = 8;               // softmax warps
-constexpr int LD_WARP0 = 10, LD_WARPS = 4;
+constexpr int LD_WARP0 = 10, LD_WARPS = 2;
 constexpr int THREADS = (LD_WARP0 + LD_WARPS) * 32;
-constexpr int O_COL = 2 * KT;             // TMEM columns: S0, S1, O
 
 template <int D>
 struct Layout {
+  static constexpr int NB = D == 256 ? 2 : 3;               // S buffers; TMEM columns: S0, S1, (S2,) O
+  static constexpr int O_COL = NB * KT;
   static constexpr int Q_BYTES = ROWS * D * 2;
   static constexpr int SLOT = 64 * D * 2;                   // half a K tile or half a V tile
-  static constexpr int SLOTS = D == 256 ? 5 : 8;
+  static constexpr int SLOTS = D == 256 ? 5 : 12;
   static constexpr int ring = Q_BYTES;
-  static constexpr int xchg = ring + SLOTS * SLOT;          // [2][2][ROWS] floats: what the column halves of a row exchange
-  static constexpr int bars = xchg + 4 * ROWS * 4;
+  static constexpr int words = ring + SLOTS * SLOT;         // [2][2][ROWS]: what the column halves of a row exchange, by parity
+  static constexpr int bars = words + 4 * ROWS * 4;
   static constexpr int total = bars + 1024;
   static_assert(total <= 232448, "shared memory");
 };
@@ -62,6 +63,7 @@ struct ItemInfo {
   int p_lo, p_hi;    // prefix keys of this part
   int o_lo, o_hi;    // own keys of this part
   int gap;           // keys that no row sees may lie between those of two sequences
+  __device__ __forceinline__ int tiles() const { return (p_hi - p_lo + KT - 1) / KT + (o_hi - o_lo + KT - 1) / KT; }   // no gap
 };
 
 struct Params {
@@ -69,6 +71,7 @@ struct Params {
   reaxmoe_attention_args a;
   int group;
   int tiles, parts, items;
+  int wide_out;      // output rows start on 32 bytes
   int* counter;      // items taken beyond the first of each pair (null when there are none)
   float* part_o;     // [parts][kv_heads][tiles * 256][D]
   float2* part_ml;   // [parts][kv_heads][tiles * 256]: maximum in units of log2, sum
@@ -145,32 +148,33 @@ __device__ __forceinline__ uint64_t desc_v(uint32_t saddr) {
 template <int D, bool BF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_kernel(const __grid_constant__ Params p) {
   using L = Layout<D>;
-  constexpr int NS = L::SLOTS;
+  constexpr int NS = L::SLOTS, NB = L::NB, AHEAD = NB - 1;   // S tiles multiplied ahead of the softmax
+  constexpr int O_COL = L::O_COL;
   constexpr float THR = BF ? 8.0f : 3.0f;     // the maximum in use may lag behind by a factor of 2^THR before O is rescaled
   // fp16 weights are shifted up by 2^12 (at most 2^15 with the lag), so that weights down to 2^-26 of the largest keep all bits
   constexpr float SHIFT = BF ? 0.0f : 12.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* xchg = reinterpret_cast<float*>(smem + L::xchg);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t* full = bars;               // [NS] (leader's) both CTAs' halves landed (tx)
   uint64_t* empty = full + NS;         // [NS] the slot's MMAs are done (commit to both CTAs)
-  uint64_t* s_full = empty + NS;       // [2] S is in TMEM (commit to both)
-  uint64_t* p_full = s_full + 2;       // [2] (leader's) P is in TMEM (16 warps of the pair)
-  uint64_t* pv_done = p_full + 2;      // [2] a tile's P V is in O (commit to both)
+  uint64_t* s_full = empty + NS;       // [NB] S is in TMEM (commit to both)
+  uint64_t* p_full = s_full + NB;      // [NB] (leader's) P is in TMEM (16 warps of the pair)
+  uint64_t* pv_done = p_full + NB;     // [2] a tile's P V is in O (commit to both)
   uint64_t* o_full = pv_done + 2;      // the item's O is complete (commit to both)
   uint64_t* o_empty = o_full + 1;      // (leader's) O has been read out (16 warps)
-  uint64_t* q_full = o_empty + 1;      // (leader's) Q rows are in shared memory (8 loader warps)
+  uint64_t* q_full = o_empty + 1;      // (leader's) Q rows are in shared memory (4 loader warps)
   uint64_t* q_empty = q_full + 1;      // the item's Q K^T are done (commit to both)
   uint64_t* info_full = q_empty + 1;   // [2] item info is there
   uint64_t* info_empty = info_full + 2;// [2] item info has been read (producer, MMA, 8 softmax warps)
   uint64_t* item_full = info_empty + 2;// the next item's number arrived (tx)
   uint64_t* item_free = item_full + 1; // (leader's) both CTAs took it
-  uint64_t* xb = item_free + 1;        // [4] the two warps of a lane quarter
+  uint64_t* xb = item_free + 1;        // [4] the two warps of a lane quarter exchange sums and flags
   uint64_t* ldb = xb + 4;              // the loader warps
   uint64_t* drainb = ldb + 1;
   ItemInfo* info = reinterpret_cast<ItemInfo*>(smem + L::bars + 512);   // [2]
   int* ld_part = reinterpret_cast<int*>(info + 2);                      // [2][LD_WARPS][7]: reductions, by parity
-  uint32_t* next_item = reinterpret_cast<uint32_t*>(ld_part + 2 * LD_WARPS * 7);
+  uint32_t* flags = reinterpret_cast<uint32_t*>(ld_part + 2 * LD_WARPS * 7);   // [2][4] rows to be done again
+  uint32_t* next_item = flags + 8;
   uint32_t* tmem_holder = next_item + 1;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
@@ -181,6 +185,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     set_status(p.a.status, REAXMOE_ERR_UNSUPPORTED);
     return;
   }
+  auto wait1 = [&](uint64_t* bar, uint32_t parity) {
+    return wait_bounded(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns);
+  };
   // every lane of a warp waits and all get the same answer
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, wait_bounded(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns)) != 0;
@@ -191,9 +198,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < NB; ++b) {
       mbar_init(smem_u32(&s_full[b]), 1);
       mbar_init(smem_u32(&p_full[b]), 2 * SM_WARPS);
+    }
+    for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&pv_done[b]), 1);
       mbar_init(smem_u32(&info_full[b]), 1);
       mbar_init(smem_u32(&info_empty[b]), SM_WARPS + 2);
@@ -210,6 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  for (int i = threadIdx.x; i < 4 * ROWS; i += THREADS) sts_volatile(smem_u32(smem + L::words) + i * 4, 1u);   // not the first use's
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -222,13 +232,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
 
   if (warp == 8) {
     // ------------------------------------------------------------------------------------------ K / V producer
-    int n = 0;                          // slots filled
-    bool ok = true;
-    auto fill = [&](bool value, int start, bool pre, int head) {
-      const int s = n % NS;
-      if (n >= NS && !wait(&empty[s], (uint32_t)(n / NS - 1))) return false;
-      const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
-      if (lane == 0) {
+    if (elect_one()) {
+      int n = 0;                          // slots filled
+      bool ok = true;
+      auto fill = [&](bool value, int start, bool pre, int head) {
+        const int s = n % NS;
+        if (n >= NS && !wait1(&empty[s], (uint32_t)(n / NS - 1))) return false;
+        const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
         const uint32_t dst = smem_u32(smem + L::ring + s * L::SLOT);
         if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * L::SLOT);
         if (!value) {
@@ -242,109 +252,132 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           for (int c = 0; c < D / 2 / W; ++c)
             tma_load_3d_pair(dst + c * (KT * W * 2), tm, bar, (int)rank * (D / 2) + c * W, head, start);
         }
+        ++n;
+        return true;
+      };
+      for (int i = 0; ok; ++i) {
+        const int ib = i & 1;
+        if (!(ok = wait1(&info_full[ib], (uint32_t)(i >> 1)))) break;
+        const ItemInfo it = info[ib];
+        mbar_arrive(smem_u32(&info_empty[ib]));
+        if (it.row0 < 0) break;
+        // K tiles run AHEAD tiles before their V tiles
+        TileIter ki, vi;
+        ki.init(p, it);
+        vi.init(p, it);
+        int ks, vs, ahead = 0;
+        bool kp, vp, more = true;
+        while (ok) {
+          if (more) more = ki.next(p, ks, kp);
+          if (more) ok = fill(false, ks, kp, it.head);
+          if (ahead < AHEAD && more) {
+            ++ahead;
+            continue;
+          }
+          if (!ok || !vi.next(p, vs, vp)) break;
+          ok = fill(true, vs, vp, it.head);
+        }
       }
-      __syncwarp();
-      ++n;
-      return true;
-    };
-    for (int i = 0; ok; ++i) {
-      const int ib = i & 1;
-      if (!(ok = wait(&info_full[ib], (uint32_t)(i >> 1)))) break;
-      const ItemInfo it = info[ib];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&info_empty[ib]));
-      if (it.row0 < 0) break;
-      TileIter ti;
-      ti.init(p, it);
-      int cur, nxt;
-      bool cpre, npre;
-      if (!ti.next(p, cur, cpre)) continue;
-      ok = fill(false, cur, cpre, it.head);
-      bool more = true;
-      while (ok && more) {
-        more = ti.next(p, nxt, npre);
-        if (more) ok = fill(false, nxt, npre, it.head);
-        if (ok) ok = fill(true, cur, cpre, it.head);
-        cur = nxt;
-        cpre = npre;
-      }
+      // let the last loads land before the CTA may exit (only matters after an abort)
+      if (rank == 0)
+        for (int f = n - 1; f >= 0 && f >= n - NS; --f) wait_drain(smem_u32(&full[f % NS]), (uint32_t)(f / NS) & 1u);
     }
-    // let the last loads land before the CTA may exit (only matters after an abort)
-    if (rank == 0)
-      for (int f = n - 1; f >= 0 && f >= n - NS; --f) wait_drain(smem_u32(&full[f % NS]), (uint32_t)(f / NS) & 1u);
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------------------ MMA issuer (leader)
-    constexpr uint32_t kFmt = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(256 >> 4) << 24);
-    constexpr uint32_t kQK = kFmt | ((uint32_t)(KT >> 3) << 17);
-    constexpr uint32_t kPV = kFmt | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // B (V) MN-major
-    int n = 0, g = 0, items = 0;        // slots consumed, tiles, items with tiles
-    bool ok = true;
-    const uint32_t qs = smem_u32(smem);
-    auto qk = [&](int tile) {
-      const int s = n % NS;
-      if (!wait(&full[s], (uint32_t)(n / NS))) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t ks = smem_u32(smem + L::ring + s * L::SLOT);
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t kFmt = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(256 >> 4) << 24);
+      constexpr uint32_t kQK = kFmt | ((uint32_t)(KT >> 3) << 17);
+      constexpr uint32_t kPV = kFmt | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // B (V) MN-major
+      const uint64_t qd = desc_sw128(smem_u32(smem)), kd = desc_sw128(smem_u32(smem + L::ring));
+      const uint64_t vd = desc_v<D>(smem_u32(smem + L::ring));
+      int slot = 0, items = 0;            // ring position, items with tiles
+      uint32_t sphase = 0;
+      int gk = 0, gv = 0;                 // tiles multiplied with K, with V
+      bool ok = true;
+      auto qk = [&]() {
+        if (!wait1(&full[slot], sphase)) return false;
+        tc_fence_after();
+        const uint64_t b = kd + (uint64_t)(slot * (L::SLOT >> 4));
+        const uint32_t d = tmem + (uint32_t)(gk % NB * KT);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_pair_ss(tmem + (tile & 1) * KT, desc_sw128(qs + c * 16384 + k * 32), desc_sw128(ks + c * 8192 + k * 32), kQK,
+            mma_pair_ss(d, qd + (uint64_t)((c * 16384 + k * 32) >> 4), b + (uint64_t)((c * 8192 + k * 32) >> 4), kQK,
                         (c | k) != 0 ? 1u : 0u);
-        commit_pair(smem_u32(&empty[s]));
-        commit_pair(smem_u32(&s_full[tile & 1]));
-      }
-      __syncwarp();
-      ++n;
-      return true;
-    };
-    for (int i = 0; ok; ++i) {
-      const int ib = i & 1;
-      if (!(ok = wait(&info_full[ib], (uint32_t)(i >> 1)))) break;
-      const ItemInfo it = info[ib];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&info_empty[ib]));
-      if (it.row0 < 0) break;
-      if (rank != 0) continue;
-      TileIter ti;
-      ti.init(p, it);
-      int start;
-      bool pre;
-      if (!ti.next(p, start, pre)) continue;
-      if (!(ok = wait(q_full, (uint32_t)items))) break;
-      if (!(ok = qk(g))) break;
-      bool more = true;
-      for (int j = 0; more; ++j, ++g) {
-        more = ti.next(p, start, pre);
-        if (more && !(ok = qk(g + 1))) break;
-        if (!more && lane == 0) commit_pair(smem_u32(q_empty));
-        if (!(ok = wait(&p_full[g & 1], (uint32_t)(g >> 1)))) break;
-        if (j == 0 && items > 0 && !(ok = wait(o_empty, (uint32_t)(items - 1)))) break;
-        const int s = n % NS;
-        if (!(ok = wait(&full[s], (uint32_t)(n / NS)))) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t vs = smem_u32(smem + L::ring + s * L::SLOT);
+        commit_pair(smem_u32(&empty[slot]));
+        commit_pair(smem_u32(&s_full[gk % NB]));
+        ++gk;
+        if (++slot == NS) {
+          slot = 0;
+          sphase ^= 1u;
+        }
+        return true;
+      };
+      for (int i = 0; ok; ++i) {
+        const int ib = i & 1;
+        if (!(ok = wait1(&info_full[ib], (uint32_t)(i >> 1)))) break;
+        const ItemInfo it = info[ib];
+        mbar_arrive(smem_u32(&info_empty[ib]));
+        if (it.row0 < 0) break;
+        TileIter ti;
+        int left = 0, start;
+        bool pre;
+        if (it.gap) ti.init(p, it); else left = it.tiles();
+        auto next = [&]() { return it.gap ? ti.next(p, start, pre) : left-- > 0; };
+        bool more = next();
+        if (!more) continue;
+        if (!(ok = wait1(q_full, (uint32_t)items))) break;
+        int ahead = 0;
+        for (; more && ahead < AHEAD; ++ahead) {
+          if (!(ok = qk())) break;
+          more = next();
+        }
+        if (!ok) break;
+        bool first = true, q_used = true;
+        while (ahead > 0) {
+          if (more) {
+            if (!(ok = qk())) break;
+            ++ahead;
+            more = next();
+          }
+          if (!more && q_used) {
+            commit_pair(smem_u32(q_empty));
+            q_used = false;
+          }
+          if (!(ok = wait1(&p_full[gv % NB], (uint32_t)(gv / NB)))) break;
+          if (first && items > 0 && !(ok = wait1(o_empty, (uint32_t)(items - 1)))) break;
+          if (!(ok = wait1(&full[slot], sphase))) break;
+          tc_fence_after();
+          const uint64_t b = vd + (uint64_t)(slot * (L::SLOT >> 4));
+          const uint32_t a = tmem + (uint32_t)(gv % NB * KT);
 #pragma unroll
           for (int k = 0; k < KT / 16; ++k)
-            mma_pair_ts(tmem + O_COL, tmem + (g & 1) * KT + k * 8, desc_v<D>(vs + k * (D == 64 ? 1024 : 2048)), kPV,
-                        (j | k) != 0 ? 1u : 0u);
-          commit_pair(smem_u32(&empty[s]));
-          commit_pair(smem_u32(&pv_done[g & 1]));
-          if (!more) commit_pair(smem_u32(o_full));
+            mma_pair_ts(tmem + O_COL, a + k * 8, b + (uint64_t)((k * (D == 64 ? 1024 : 2048)) >> 4), kPV,
+                        first && k == 0 ? 0u : 1u);
+          commit_pair(smem_u32(&empty[slot]));
+          commit_pair(smem_u32(&pv_done[gv & 1]));
+          if (ahead == 1) commit_pair(smem_u32(o_full));
+          first = false;
+          ++gv;
+          --ahead;
+          if (++slot == NS) {
+            slot = 0;
+            sphase ^= 1u;
+          }
         }
-        __syncwarp();
-        ++n;
+        ++items;
       }
-      ++items;
-    }
-    // every issued MMA has completed before TMEM may be released (matters after an abort)
-    if (rank == 0) {
-      if (lane == 0)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drainb)) : "memory");
-      __syncwarp();
+      // every issued MMA has completed before TMEM may be released (matters after an abort)
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(drainb)) : "memory");
       wait_drain(smem_u32(drainb), 0);
+    } else if (rank != 0 && lane == 0) {
+      for (int i = 0;; ++i) {
+        if (!wait1(&info_full[i & 1], (uint32_t)(i >> 1))) break;
+        const int row0 = info[i & 1].row0;
+        mbar_arrive(smem_u32(&info_empty[i & 1]));
+        if (row0 < 0) break;
+      }
     }
   } else if (warp >= LD_WARP0) {
     // ------------------------------------------------------------------------------------------ loader: items and Q rows
@@ -379,11 +412,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       // later tiles first: of a causal sequence these are the long ones
       const int part = item % p.parts, head = (item / p.parts) % p.a.kv_heads;
       const int row0 = (p.tiles - 1 - item / p.parts / p.a.kv_heads) * 2 * ROWS;
-      // the union of the 256 rows' ranges: thread = rows 2 tid, 2 tid + 1
-      int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0, gap = 0, first_lo = INT_MAX, last_hi = INT_MAX;
+      // the union of the 256 rows' ranges: thread = rows RPT tid ... RPT tid + RPT - 1
+      constexpr int RPT = 2 * ROWS / (LD_WARPS * 32);
+      int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0, gap = 0, first_lo = -1, last_hi = INT_MAX;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = row0 + 2 * tid + h;
+      for (int h = 0; h < RPT; ++h) {
+        const int r = row0 + RPT * tid + h;
         if (r < nrows) {
           const RowKeys rk = row_keys(p.a, r / p.group);
           if (rk.p_lo < rk.p_hi) {
@@ -397,8 +431,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           if (h == 0) first_lo = rk.k_lo;
           else if (rk.k_lo - last_hi >= KT) gap = 1;
           last_hi = rk.k_hi;
-        } else if (h == 0) {
-          first_lo = -1;
         }
       }
       const int nx = __shfl_down_sync(0xffffffffu, first_lo, 1);
@@ -433,8 +465,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         klo = min(klo, all[w * 7 + 2]);
         khi = max(khi, all[w * 7 + 3]);
         gap |= all[w * 7 + 4];
-        if (w > 0 && all[w * 7 - 1] != INT_MAX && all[w * 7 + 5] >= 0 && all[w * 7 + 5] != INT_MAX &&
-            all[w * 7 + 5] - all[w * 7 - 1] >= KT)
+        if (w > 0 && all[w * 7 - 1] != INT_MAX && all[w * 7 + 5] >= 0 && all[w * 7 + 5] - all[w * 7 - 1] >= KT)
           gap = 1;
       }
       if (p.counter != nullptr && i > 0 && tid == 0) mbar_arrive_cluster(leader_free);   // all loader threads have read it
@@ -460,11 +491,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       bool pre;
       if (!ti.next(p, start, pre)) continue;
       if (items > 0 && !wait(q_empty, (uint32_t)(items - 1))) break;
-      // 8 threads copy 128 bytes (64 elements) of a row; 16 rows per pass
+      // 8 threads copy 128 bytes (64 elements) of a row
       const int piece = tid & 7;
-#pragma unroll 1
-      for (int j = 0; j < ROWS / 16; ++j) {
-        const int r = j * 16 + (tid >> 3);
+      constexpr int RPP = LD_WARPS * 4;          // rows per pass
+#pragma unroll 2
+      for (int j = 0; j < ROWS / RPP; ++j) {
+        const int r = j * RPP + (tid >> 3);
         const int row = row0 + (int)rank * ROWS + r;
         const uint32_t dst = smem_u32(smem) + r * 128 + ((piece ^ (r & 7)) << 4);
         if (row < nrows) {
@@ -490,168 +522,274 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t ocol = tmem + lanes + O_COL;
     const int nrows = row_count(p);
     const float c = p.a.scale * 1.4426950408889634f;
-    const uint32_t leader_p[2] = {map_to_rank(smem_u32(&p_full[0]), 0), map_to_rank(smem_u32(&p_full[1]), 0)};
-    const uint32_t leader_o = map_to_rank(smem_u32(o_empty), 0);
-    int g = 0, items = 0, ex = 0;
+    const f32x2 c2 = x2_pack(c, c);
+    const uint32_t p_full0 = map_to_rank(smem_u32(&p_full[0]), 0), leader_o = map_to_rank(smem_u32(o_empty), 0);
+    const uint32_t x_mine = smem_u32(smem + L::words) + (uint32_t)(half * ROWS + r) * 4;
+    const uint32_t x_other = smem_u32(smem + L::words) + (uint32_t)((half ^ 1) * ROWS + r) * 4;
+    int g = 0, items = 0, ex = 0, x_n = 0;
     bool ok = true;
-    // the value of the row's other column half (both warps of the quarter call it)
-    auto exchange = [&](float mine, float& other) {
-      float* buf = xchg + (ex & 1) * 2 * ROWS;
-      buf[half * ROWS + r] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&xb[quarter]));
-      const bool fine = wait(&xb[quarter], (uint32_t)ex);
-      other = buf[(half ^ 1) * ROWS + r];
-      ++ex;
-      return fine;
-    };
-    for (int i = 0; ok; ++i) {
+
+    ItemInfo it, it_next;
+    RowKeys rk, rk_next;
+    int tok = 0, tok_next = 0;
+    // the next item, and what this thread's row of it sees. A row that is not there needs no mask: its sums are not read.
+    auto fetch = [&](int i) {
       const int ib = i & 1;
-      if (!(ok = wait(&info_full[ib], (uint32_t)(i >> 1)))) break;
-      const ItemInfo it = info[ib];
+      if (!wait(&info_full[ib], (uint32_t)(i >> 1))) return false;
+      it_next = info[ib];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&info_empty[ib]));
+      const int row = it_next.row0 + (int)rank * ROWS + r;
+      rk_next = {0, INT_MAX, 0, INT_MAX};
+      tok_next = 0;
+      if (it_next.row0 >= 0 && row < nrows) {
+        tok_next = row / p.group;
+        rk_next = row_keys(p.a, tok_next);
+      }
+      return true;
+    };
+    // both warps of a lane quarter meet: what each wrote to shared memory before is there for the other afterwards
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&xb[quarter]));
+      return wait(&xb[quarter], (uint32_t)ex++);
+    };
+    // The halves of a row exchange a value (maximum, sum) through one word each, whose lowest bit says which use of the word it
+    // is: a word is used every other time, and written again only after the other side has gone on to the next one. Both
+    // sides go on with the same two words, without that bit.
+    auto post = [&](float v) {
+      sts_volatile(x_mine + (uint32_t)((x_n & 1) * 2 * ROWS * 4), (__float_as_uint(v) & ~1u) | (uint32_t)((x_n >> 1) & 1));
+    };
+    auto receive = [&](float& other) {
+      const uint32_t at = x_other + (uint32_t)((x_n & 1) * 2 * ROWS * 4), tag = (uint32_t)((x_n >> 1) & 1);
+      ++x_n;
+      uint32_t v = lds_volatile(at);
+      uint64_t t0 = 0;
+      for (uint32_t n = 1; !__all_sync(0xffffffffu, (v & 1u) == tag); ++n) {
+        if ((n & 63u) == 0u) {
+          if (t0 == 0) t0 = globaltimer();
+          const bool late = globaltimer() - t0 > p.timeout_ns;
+          if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
+            if (late) set_status(p.a.status, REAXMOE_ERR_DEVICE_TIMEOUT);
+            *abort_flag = 1;
+            return false;
+          }
+        }
+        v = lds_volatile(at);
+      }
+      other = __uint_as_float(v & ~1u);
+      return true;
+    };
+    auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & ~1u); };   // as the other side gets it
+    // 32 scores -> weights 2^(c s - mc), their sums, and the packed weights to 16 TMEM columns. seen: bit x for column x
+    auto weights = [&](uint32_t (&s)[32], uint32_t seen, float mc, f32x2 (&sum)[2], uint32_t dst) {
+      uint32_t w[16];
+      if (__any_sync(0xffffffffu, seen != 0u)) {
+        const f32x2 nm = x2_pack(-mc, -mc);
+        if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) s[x] = (seen >> x) & 1u ? s[x] : 0xFF800000u;
+        }
+#pragma unroll
+        for (int x = 0; x < 32; x += 2) {
+          float e0, e1;
+          x2_unpack(x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm), e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          w[x / 2] = pack2<BF>(e0, e1);
+          sum[(x / 2) & 1] = x2_add(sum[(x / 2) & 1], x2_pack(e0, e1));
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) w[x] = 0u;
+      }
+      tc_st_32x32b_x16(dst, w);
+    };
+    auto chunk_max = [&](const uint32_t (&s)[32], uint32_t seen, float (&mx)[2]) {
+      if (__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          mx[0] = max3(mx[0], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+          mx[1] = max3(mx[1], __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 32; ++x) mx[x & 1] = fmaxf(mx[x & 1], (seen >> x) & 1u ? __uint_as_float(s[x]) : -INFINITY);
+      }
+    };
+
+    if (!fetch(0)) ok = false;
+    for (int i = 0; ok; ++i) {
+      it = it_next;
+      rk = rk_next;
+      tok = tok_next;
       if (it.row0 < 0) break;
       const int row = it.row0 + (int)rank * ROWS + r;
       const bool live = row < nrows;
       const bool any_live = __any_sync(0xffffffffu, live);
-      const int tok = live ? row / p.group : 0;
-      // a row that is not there needs no mask (its sums are not read)
-      RowKeys rk = {0, INT_MAX, 0, INT_MAX};
-      if (live) rk = row_keys(p.a, tok);
       const bool none = rk.p_lo >= rk.p_hi && rk.k_lo >= rk.k_hi;
-      float m = -INFINITY, l = 0.0f;       // the maximum in use (of scores times c) and this half's sum
+      float m = -INFINITY, l = 0.0f;             // the maximum in use (of scores times c), the sum of this half's weights
       TileIter ti;
       ti.init(p, it);
-      int start, j = 0;
-      bool pre;
-      for (; ti.next(p, start, pre); ++j, ++g) {
+      int j = 0;
+      // a tile: which of this thread's 64 columns its row sees, and whether any row of the warp sees any of the 128
+      struct Tile { uint32_t seen0, seen1; bool some; } cur;
+      auto next = [&](Tile& t) {
+        int start;
+        bool pre;
+        if (!ti.next(p, start, pre)) return false;
         // keys from the part's end on are the next part's, whose first tile may begin inside this one where there are gaps
         const int lo = pre ? rk.p_lo : rk.k_lo, hi = pre ? min(rk.p_hi, it.p_hi) : min(rk.k_hi, it.o_hi);
         const int a0 = max(lo - start, 0), a1 = hi - start;          // columns [a0, a1) are seen
-        if (!(ok = wait(&s_full[g & 1], (uint32_t)(g >> 1)))) break;
-        const uint32_t scol = tmem + lanes + (uint32_t)((g & 1) * KT);
-        if (any_live) {
+        auto seen = [&](int col) {                                   // of columns col .. col + 31
+          const int f = min(max(a0 - col, 0), 32), e = min(max(a1 - col, 0), 32);
+          const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_f = f == 32 ? 0xffffffffu : (1u << f) - 1u;
+          return below_e & ~below_f;
+        };
+        t.seen0 = seen(half * 64);
+        t.seen1 = seen(half * 64 + 32);
+        t.some = __any_sync(0xffffffffu, a0 < KT && a1 > a0);
+        return true;
+      };
+      uint32_t s0[32], s1[32];
+      float mine = -INFINITY;
+      auto scol = [&](int tile) { return tmem + lanes + (uint32_t)(tile % NB * KT); };
+      auto load = [&](int tile, uint32_t (&x0)[32], uint32_t (&x1)[32]) {   // of the tile's scores, this half's columns
+        tc_fence_after();
+        tc_ld_32x32b_x32(scol(tile) + half * 64, x0);
+        tc_ld_32x32b_x32(scol(tile) + half * 64 + 32, x1);
+      };
+      auto find_max = [&](const Tile& t, uint32_t (&x0)[32], uint32_t (&x1)[32]) {
+        tc_wait_ld(x0);
+        loaded(x1);
+        float mx[2] = {-INFINITY, -INFINITY};
+        chunk_max(x0, t.seen0, mx);
+        chunk_max(x1, t.seen1, mx);
+        mine = cut(fmaxf(mx[0], mx[1]));
+        post(mine);
+      };
+      // the softmax of one tile whose scores are in registers and whose half maxima are posted
+      auto weigh = [&](const Tile& t, uint32_t (&x0)[32], uint32_t (&x1)[32]) {
+        float top;
+        if (!receive(top)) return false;
+        top = fmaxf(top, mine) * c;
+        const bool grow = top - m > THR;         // from -inf on the first key
+        const bool rescale = grow && m != -INFINITY;
+        if (__any_sync(0xffffffffu, rescale)) {
+          const float f = rescale ? ex2(m - top) : 1.0f;
+          l *= f;
+          if (!wait(&pv_done[(g - 1) & 1], (uint32_t)((g - 1) >> 1))) return false;
           tc_fence_after();
-          const bool all = __all_sync(0xffffffffu, a0 == 0 && a1 >= KT);
-          const bool nothing = __all_sync(0xffffffffu, a0 >= KT || a1 <= a0);
-          uint32_t w[32];
-          if (nothing) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x) w[x] = 0u;
-          } else {
-            uint32_t s0[32], s1[32];
-            tc_ld_32x32b_x32(scol + half * 64, s0);
-            tc_ld_32x32b_x32(scol + half * 64 + 32, s1);
-            tc_wait_ld();
-            if (!all) {
-              const int b0 = a0 - half * 64, b1 = a1 - half * 64;
-#pragma unroll
-              for (int x = 0; x < 32; ++x) {
-                if (x < b0 || x >= b1) s0[x] = 0xFF800000u;
-                if (x + 32 < b0 || x + 32 >= b1) s1[x] = 0xFF800000u;
-              }
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              mx[0] = fmaxf(mx[0], __uint_as_float(s0[x]));
-              mx[1] = fmaxf(mx[1], __uint_as_float(s0[x + 1]));
-              mx[2] = fmaxf(mx[2], __uint_as_float(s1[x]));
-              mx[3] = fmaxf(mx[3], __uint_as_float(s1[x + 1]));
-            }
-            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), theirs;
-            if (!(ok = exchange(top, theirs))) break;
-            top = fmaxf(top, theirs) * c;
-            const bool grow = top - m > THR;       // from -inf on the first key
-            const bool rescale = grow && m != -INFINITY;
-            const float f = rescale ? ex2(m - top) : 1.0f;
-            if (grow) m = top;
-            l *= f;
-            if (j > 0 && __any_sync(0xffffffffu, rescale)) {
-              if (!(ok = wait(&pv_done[(g - 1) & 1], (uint32_t)((g - 1) >> 1)))) break;
-              tc_fence_after();
-              constexpr int HC = D / 2;            // this half's columns of O
+          constexpr int HC = D / 2;              // this half's columns of O
 #pragma unroll 1
-              for (int x = 0; x < HC; x += 32) {
-                uint32_t o[32];
-                tc_ld_32x32b_x32(tmem + lanes + O_COL + half * HC + x, o);
-                tc_wait_ld();
+          for (int x = 0; x < HC; x += 32) {
+            uint32_t o[32];
+            tc_ld_32x32b_x32(ocol + half * HC + x, o);
+            tc_wait_ld(o);
 #pragma unroll
-                for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                tc_st_32x32b_x32(tmem + lanes + O_COL + half * HC + x, o);
-              }
-              tc_wait_st();
-            }
-            const float mc = (m == -INFINITY ? 0.0f : m) - SHIFT;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              const float e0 = ex2(fmaf(__uint_as_float(s0[x]), c, -mc)), e1 = ex2(fmaf(__uint_as_float(s0[x + 1]), c, -mc));
-              w[x / 2] = pack2<BF>(e0, e1);
-              sum[0] += e0;
-              sum[1] += e1;
-            }
-#pragma unroll
-            for (int x = 0; x < 32; x += 2) {
-              const float e0 = ex2(fmaf(__uint_as_float(s1[x]), c, -mc)), e1 = ex2(fmaf(__uint_as_float(s1[x + 1]), c, -mc));
-              w[16 + x / 2] = pack2<BF>(e0, e1);
-              sum[2] += e0;
-              sum[3] += e1;
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            tc_st_32x32b_x32(ocol + half * HC + x, o);
           }
-          tc_st_32x32b_x32(scol + half * 32, w);
+        }
+        if (grow) m = top;
+        const float mc = (m == -INFINITY ? 0.0f : m) - SHIFT;
+        f32x2 sum[2] = {0ull, 0ull};
+        // P takes the place of the first 64 columns of S, which both halves have read
+        weights(x0, t.seen0, mc, sum, scol(g) + half * 32);
+        weights(x1, t.seen1, mc, sum, scol(g) + half * 32 + 16);
+        float y0, y1;
+        x2_unpack(x2_add(sum[0], sum[1]), y0, y1);
+        l += y0 + y1;
+        return true;
+      };
+      auto nothing = [&]() {                     // no row of the warp sees any key of the tile
+        uint32_t z[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) z[x] = 0u;
+        tc_st_32x32b_x16(scol(g) + half * 32, z);
+        tc_st_32x32b_x16(scol(g) + half * 32 + 16, z);
+      };
+      auto done = [&]() {
+        if (any_live) {
           tc_wait_st();
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_p[g & 1]);
+        if (lane == 0) mbar_arrive_cluster(p_full0 + (uint32_t)(g % NB * 8));
+        ++g;
+        ++j;
+      };
+      while (next(cur)) {
+        if (!(ok = wait(&s_full[g % NB], (uint32_t)(g / NB)))) break;
+        if (any_live) {
+          if (cur.some) {
+            load(g, s0, s1);
+            find_max(cur, s0, s1);
+            if (!(ok = weigh(cur, s0, s1))) break;
+          } else {
+            nothing();
+          }
+        }
+        done();
       }
       if (!ok) break;
+      if (!(ok = fetch(i + 1))) break;           // while the last products run
       // the item's rows: o = O / l, or the partial sums of this part
-      float other = 0.0f;
-      if (j > 0 && !(ok = wait(o_full, (uint32_t)items))) break;
       if (any_live) {
-        if (!(ok = exchange(l, other))) break;
-        l += other;
+        float other;
+        post(l);
+        if (!(ok = receive(other))) break;
+        l = cut(l) + other;
+        if (j > 0 && !(ok = wait(o_full, (uint32_t)items))) break;
+        tc_fence_after();
         constexpr int HC = D / 2;
         const int head = it.head * p.group + (row - tok * p.group);
         const int64_t part_row = ((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * ROWS) + row;
         const float inv = none ? 0.0f : 1.0f / l;
+        const f32x2 inv2 = x2_pack(inv, inv);
         uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride + half * HC;
-        bool bad = false;
-        if (j > 0) tc_fence_after();
-#pragma unroll 1
+        f32x2 check = 0ull;                      // becomes NaN with the first value that is not finite
+#pragma unroll
         for (int x = 0; x < HC; x += 32) {
           uint32_t o[32];
           if (j > 0) {
-            tc_ld_32x32b_x32(tmem + lanes + O_COL + half * HC + x, o);
-            tc_wait_ld();
+            tc_ld_32x32b_x32(ocol + half * HC + x, o);
+            tc_wait_ld(o);
           } else {
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = 0u;
           }
-          if (live && p.parts > 1) {
+          if (p.parts > 1) {
             float4* dst = reinterpret_cast<float4*>(p.part_o + part_row * D + half * HC + x);
+            if (live) {
 #pragma unroll
-            for (int y = 0; y < 8; ++y)
-              dst[y] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]), __uint_as_float(o[4 * y + 2]),
-                                   __uint_as_float(o[4 * y + 3]));
-          } else if (live) {
+              for (int y = 0; y < 8; ++y)
+                dst[y] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]), __uint_as_float(o[4 * y + 2]),
+                                     __uint_as_float(o[4 * y + 3]));
+            }
+          } else {
+            uint32_t v[2][8];
 #pragma unroll
-            for (int y = 0; y < 32; y += 8) {
-              uint32_t v[4];
+            for (int y = 0; y < 32; y += 2) {
+              const f32x2 z = x2_mul(x2_pack(__uint_as_float(o[y]), __uint_as_float(o[y + 1])), inv2);
+              check = x2_fma(z, 0ull, check);
+              float z0, z1;
+              x2_unpack(z, z0, z1);
+              v[y / 16][(y / 2) & 7] = pack2<BF>(z0, z1);
+            }
+            if (live) {
+              if (p.wide_out) {
+                st_global_v8(out + x, v[0]);
+                st_global_v8(out + x + 16, v[1]);
+              } else {
 #pragma unroll
-              for (int z = 0; z < 4; ++z) {
-                const float f0 = none ? 0.0f : __uint_as_float(o[y + 2 * z]) * inv;
-                const float f1 = none ? 0.0f : __uint_as_float(o[y + 2 * z + 1]) * inv;
-                bad |= !(fabsf(f0) < INFINITY) || !(fabsf(f1) < INFINITY);
-                v[z] = pack2<BF>(f0, f1);
+                for (int y = 0; y < 4; ++y)
+                  *reinterpret_cast<uint4*>(out + x + y * 8) =
+                      make_uint4(v[y / 2][(y & 1) * 4], v[y / 2][(y & 1) * 4 + 1], v[y / 2][(y & 1) * 4 + 2], v[y / 2][(y & 1) * 4 + 3]);
               }
-              *reinterpret_cast<uint4*>(out + x + y) = make_uint4(v[0], v[1], v[2], v[3]);
             }
           }
           __syncwarp();
@@ -659,22 +797,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         tc_fence_before();
         __syncwarp();
         if (j > 0 && lane == 0) mbar_arrive_cluster(leader_o);
-        if (p.parts > 1) {
-          if (live && half == 0) p.part_ml[part_row] = make_float2(m, l);
-        } else {
-          if (live && half == 0 && p.a.lse != nullptr)
-            p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
-          // 0 x (an infinity or NaN of a value that the row does not see) is NaN: such rows are done again key by key. A sum
-          // that is NaN itself came from a key that the row does see.
-          if (!(ok = exchange(bad && l == l ? 1.0f : 0.0f, other))) break;
-          uint32_t again = __ballot_sync(0xffffffffu, live && ((bad && l == l) || other != 0.0f));
-          while (half == 0 && again != 0u) {
-            const int src = __ffs(again) - 1;
-            again &= again - 1u;
-            row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src));
+        // 0 x (an infinity or NaN of a value that the row does not see) is NaN: such rows are done again key by key. A sum
+        // that is NaN itself came from a key that the row does see.
+        float x0, x1;
+        x2_unpack(check, x0, x1);
+        const uint32_t mine = __ballot_sync(0xffffffffu, live && l == l && !(x0 + x1 == 0.0f));
+        if (lane == 0) flags[half * 4 + quarter] = mine;
+        if (!(ok = meet())) break;
+        if (half == 0) {
+          if (p.parts > 1) {
+            if (live) p.part_ml[part_row] = make_float2(m, l);
+          } else {
+            if (live && p.a.lse != nullptr)
+              p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
+            uint32_t again = mine | flags[4 + quarter];
+            while (again != 0u) {
+              const int src = __ffs(again) - 1;
+              again &= again - 1u;
+              row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src));
+            }
           }
         }
       } else if (j > 0) {
+        if (!(ok = wait(o_full, (uint32_t)items))) break;
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(leader_o);
       }
@@ -793,6 +938,7 @@ static int launch_t(const AttentionLaunch& l, const Plan& pl, cudaStream_t s) {
   p.tiles = pl.tiles;
   p.parts = pl.parts;
   p.items = pl.items;
+  p.wide_out = ((reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && (a.out_stride & 15) == 0 && (a.out_head_stride & 15) == 0) ? 1 : 0;
   uint8_t* ws = static_cast<uint8_t*>(l.workspace);
   p.counter = pl.items > pl.pairs ? reinterpret_cast<int*>(ws) : nullptr;
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);

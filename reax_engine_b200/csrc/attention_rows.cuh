@@ -57,7 +57,10 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (BF) return pack_bf16x2(lo, hi);
+  if constexpr (BF) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);    // one conversion instruction for the pair
+    return *reinterpret_cast<const uint32_t*>(&b);
+  }
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }

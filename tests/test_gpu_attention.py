@@ -149,6 +149,18 @@ def test_many_rows_split_and_whole_agree():
     run((1,) * 6, (3,) * 6, hq=4, hk=1, d=256, prefix=3000, seed=4)
 
 
+def test_more_tiles_than_pairs():
+    """More row tiles than CTA pairs, the last of them nearly empty, so that every pair works through several."""
+    import reax_engine_b200 as R
+    for d, dtype, lens in ((64, "bf16", (700, 1, 0, 900, 401)), (256, "fp16", (1300, 37))):
+        c = cu(lens)
+        q, k, v, _, _ = tensors(c[-1], c[-1], 16, 16, d, dtype, 6)
+        o, lse = R.prompt_attention(q, k, v, dev(c), return_lse=True)
+        for h in (0, 9, 15):
+            one = [t[:, h:h + 1] for t in (q, k, v)]
+            check(o[:, h:h + 1], reference(*one, c, c, d ** -0.5), lse[:, h:h + 1])
+
+
 def test_large_and_small_scores():
     """Scores of hundreds, whose running maximum grows from tile to tile, and weights far below the largest."""
     import reax_engine_b200 as R
