@@ -195,7 +195,7 @@ typedef struct reaxmoe_attention_args {
   int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
   int64_t prefix_k_stride, prefix_k_head_stride, prefix_v_stride, prefix_v_head_stride, out_stride, out_head_stride;
   int64_t q_tokens, k_tokens, prefix;   /* prefix + k_tokens < 2^31 - 2^16, q_tokens * q_heads / kv_heads < 2^31 - 2^16 */
-  int32_t seqs, q_heads, kv_heads, head_dim;   /* q_heads a multiple of kv_heads; head_dim 64, 128 or 256 */
+  int32_t seqs, q_heads, kv_heads, head_dim;   /* q_heads a multiple (<= 128) of kv_heads; head_dim 64, 128 or 256 */
   int32_t dtype;              /* REAXMOE_BF16 or REAXMOE_FP16 */
   int32_t causal;             /* 0 or 1 */
   int32_t window;             /* 0: none; else >= 1, with causal */

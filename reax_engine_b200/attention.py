@@ -105,7 +105,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                      window: int | None = None, return_lse: bool = False, out: torch.Tensor | None = None,
                      workspace: torch.Tensor | None = None, status: torch.Tensor | None = None):
     """Attention of packed sequences: q [tokens, heads, d], k / v [key tokens, kv_heads, d], bf16 or fp16, d 64, 128 or 256,
-    heads a multiple of kv_heads (query head h reads KV head h // (heads / kv_heads)). Sequence b holds query rows
+    heads a multiple (at most 128) of kv_heads (query head h reads KV head h // (heads / kv_heads)). Sequence b holds query rows
     [cu_seqlens[b], cu_seqlens[b + 1]) and keys [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (default: the same); the cumulative
     lengths are int32 on the device, and nothing is read back from it.
 

@@ -450,6 +450,8 @@ static int check_attention_sizes(const reaxmoe_attention_args* a) {
   if (a->q_heads < 1 || a->kv_heads < 1 || a->kv_heads > 65535 || a->q_heads % a->kv_heads != 0)
     return fail(REAXMOE_ERR_BAD_SHAPE, "attention: q_heads=%d must be a multiple of kv_heads=%d (at most 65535)", a->q_heads,
                 a->kv_heads);
+  if (a->q_heads / a->kv_heads > 128)
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: %d query heads per KV head (at most 128)", a->q_heads / a->kv_heads);
   if (a->seqs < 0 || a->q_tokens < 0 || a->k_tokens < 0 || a->prefix < 0 || a->q_tokens > kMax || a->k_tokens > kMax ||
       a->prefix > kMax || a->prefix + a->k_tokens > kMax || a->q_tokens * (a->q_heads / a->kv_heads) > kMax)
     return fail(REAXMOE_ERR_BAD_SHAPE, "attention: seqs=%d q_tokens=%lld k_tokens=%lld prefix=%lld out of range", a->seqs,

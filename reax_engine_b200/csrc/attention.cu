@@ -5,8 +5,8 @@
 //   row i sees, m_i a running maximum (one pass over the keys; o and the sum are rescaled when it grows).
 //
 // Rows. Query head h of KV head g reads the same keys as its group's other heads, so the rows of KV head g are (token, head of
-// the group) pairs, row = token * group + h % group, over ALL packed tokens: a tile of 256 consecutive rows (128 in each CTA of
-// a pair) may end one sequence, hold others whole and begin the next. What a row sees is two ranges of keys (of the prefix and
+// the group) pairs, row = token * group + h % group, over ALL packed tokens: a tile of up to 256 consecutive rows (the whole
+// tokens that fit into 128 rows, in each CTA of a pair) may end one sequence, hold others whole and begin the next. What a row sees is two ranges of keys (of the prefix and
 // of its own sequence), a tile goes over the union of its rows' ranges, and the mask of a row is two comparisons with its
 // range. Packing rows across sequences is what computes a shared prefix once for a batch of short continuations, and it reads
 // the keys of a batch of single tokens once per KV head; for long prompts it costs nothing over tiles that stop at a sequence's
@@ -24,7 +24,7 @@
 //   warps 0..7    softmax: TMEM lane quarter w % 4 (thread = row), column half w / 4; the halves of a row exchange maxima
 //   warp 8        K / V producer: ring of slots, alternately half a K tile (64 keys x D) and half a V tile (128 keys x D / 2)
 //   warp 9        allocates TMEM; in the leader CTA one thread issues all MMAs of the pair
-//   warps 10, 11  loader: takes the next item, works out its key ranges, copies its Q rows
+//   warp 10       loader: takes the next item, works out its key ranges, loads its Q rows (TMA)
 // Items (row tile, KV head, part of the keys) are taken in order, the first by pair number, further ones from a counter.
 // With few rows an item's keys are split over several pairs, which leave partial sums that combine_kernel joins.
 // All waits are bounded (globaltimer); a timeout records REAXMOE_ERR_DEVICE_TIMEOUT and the CTA winds down.
@@ -40,8 +40,7 @@ namespace attn {
 constexpr int ROWS = 128;                 // query rows per CTA
 constexpr int KT = 128;                   // keys per tile
 constexpr int SM_WARPS = 8;               // softmax warps
-constexpr int LD_WARP0 = 10, LD_WARPS = 2;
-constexpr int THREADS = (LD_WARP0 + LD_WARPS) * 32;
+constexpr int THREADS = (SM_WARPS + 3) * 32;
 
 template <int D>
 struct Layout {
@@ -59,6 +58,7 @@ struct Layout {
 
 struct ItemInfo {
   int row0;          // first row of the pair's tile; -1: no more items
+  int b0, b1;        // first and last sequence that has rows in it
   int head, part;    // KV head, part of the keys
   int p_lo, p_hi;    // prefix keys of this part
   int o_lo, o_hi;    // own keys of this part
@@ -67,14 +67,15 @@ struct ItemInfo {
 };
 
 struct Params {
-  CUtensorMap tmK, tmV, tmPK, tmPV;
+  CUtensorMap tmQ, tmK, tmV, tmPK, tmPV;
   reaxmoe_attention_args a;
   int group;
+  int rows;          // rows of a CTA's tile: group times the tokens that fit into 128
   int tiles, parts, items;
   int wide_out;      // output rows start on 32 bytes
   int* counter;      // items taken beyond the first of each pair (null when there are none)
-  float* part_o;     // [parts][kv_heads][tiles * 256][D]
-  float2* part_ml;   // [parts][kv_heads][tiles * 256]: maximum in units of log2, sum
+  float* part_o;     // [parts][kv_heads][tiles * 2 * rows][D]
+  float2* part_ml;   // [parts][kv_heads][tiles * 2 * rows]: maximum in units of log2, sum
   unsigned long long timeout_ns;
 };
 
@@ -107,9 +108,9 @@ struct TileIter {
     gap = it.gap != 0;
     if (gap) {
       t0 = it.row0 / p.group;
-      t1 = (min(it.row0 + 2 * ROWS, row_count(p)) - 1) / p.group + 1;
-      b = sequence_of(p.a, t0);
-      b_end = sequence_of(p.a, t1 - 1);
+      t1 = min(it.row0 + 2 * p.rows, row_count(p)) / p.group;
+      b = it.b0;
+      b_end = it.b1;
       need(p.a);
     }
   }
@@ -162,18 +163,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   uint64_t* pv_done = p_full + NB;     // [2] a tile's P V is in O (commit to both)
   uint64_t* o_full = pv_done + 2;      // the item's O is complete (commit to both)
   uint64_t* o_empty = o_full + 1;      // (leader's) O has been read out (16 warps)
-  uint64_t* q_full = o_empty + 1;      // (leader's) Q rows are in shared memory (4 loader warps)
+  uint64_t* q_full = o_empty + 1;      // (leader's) both CTAs' Q rows landed (tx)
   uint64_t* q_empty = q_full + 1;      // the item's Q K^T are done (commit to both)
   uint64_t* info_full = q_empty + 1;   // [2] item info is there
   uint64_t* info_empty = info_full + 2;// [2] item info has been read (producer, MMA, 8 softmax warps)
   uint64_t* item_full = info_empty + 2;// the next item's number arrived (tx)
   uint64_t* item_free = item_full + 1; // (leader's) both CTAs took it
   uint64_t* xb = item_free + 1;        // [4] the two warps of a lane quarter exchange sums and flags
-  uint64_t* ldb = xb + 4;              // the loader warps
-  uint64_t* drainb = ldb + 1;
+  uint64_t* drainb = xb + 4;
   ItemInfo* info = reinterpret_cast<ItemInfo*>(smem + L::bars + 512);   // [2]
-  int* ld_part = reinterpret_cast<int*>(info + 2);                      // [2][LD_WARPS][7]: reductions, by parity
-  uint32_t* flags = reinterpret_cast<uint32_t*>(ld_part + 2 * LD_WARPS * 7);   // [2][4] rows to be done again
+  uint32_t* flags = reinterpret_cast<uint32_t*>(info + 2);              // [2][4] rows to be done again
   uint32_t* next_item = flags + 8;
   uint32_t* tmem_holder = next_item + 1;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -209,12 +208,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     }
     mbar_init(smem_u32(o_full), 1);
     mbar_init(smem_u32(o_empty), 2 * SM_WARPS);
-    mbar_init(smem_u32(q_full), 2 * LD_WARPS);
+    mbar_init(smem_u32(q_full), 1);
     mbar_init(smem_u32(q_empty), 1);
     mbar_init(smem_u32(item_full), 1);
     mbar_init(smem_u32(item_free), 2);
     for (int b = 0; b < 4; ++b) mbar_init(smem_u32(&xb[b]), 2);
-    mbar_init(smem_u32(ldb), LD_WARPS);
     mbar_init(smem_u32(drainb), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -345,9 +343,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
             commit_pair(smem_u32(q_empty));
             q_used = false;
           }
-          if (!(ok = wait1(&p_full[gv % NB], (uint32_t)(gv / NB)))) break;
-          if (first && items > 0 && !(ok = wait1(o_empty, (uint32_t)(items - 1)))) break;
           if (!(ok = wait1(&full[slot], sphase))) break;
+          if (first && items > 0 && !(ok = wait1(o_empty, (uint32_t)(items - 1)))) break;
+          if (!(ok = wait1(&p_full[gv % NB], (uint32_t)(gv / NB)))) break;
           tc_fence_after();
           const uint64_t b = vd + (uint64_t)(slot * (L::SLOT >> 4));
           const uint32_t a = tmem + (uint32_t)(gv % NB * KT);
@@ -379,31 +377,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         if (row0 < 0) break;
       }
     }
-  } else if (warp >= LD_WARP0) {
+  } else if (warp == 10) {
     // ------------------------------------------------------------------------------------------ loader: items and Q rows
-    const int lw = warp - LD_WARP0, tid = threadIdx.x - LD_WARP0 * 32;
-    const int nrows = row_count(p);
-    const uint32_t leader_q = map_to_rank(smem_u32(q_full), 0), leader_free = map_to_rank(smem_u32(item_free), 0);
-    int items = 0, syncs = 0;
+    const int ntok = row_count(p) / p.group, per = p.rows / p.group;      // tokens; tokens of a CTA's tile
+    int items = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       int item = i == 0 ? pair : p.items;
       if (i > 0 && p.counter != nullptr) {
-        if (rank == 0 && tid == 0) {
-          if (i <= 1 || wait_bounded(smem_u32(item_free), (uint32_t)(i - 2) & 1u, abort_flag, p.a.status, p.timeout_ns)) {
+        if (lane == 0) {
+          if (rank == 0 && (i == 1 || wait1(item_free, (uint32_t)(i - 2)))) {
             const uint32_t v = (uint32_t)(pairs + atomicAdd(p.counter, 1));
             for (uint32_t r = 0; r < 2; ++r)
               st_async_u32(map_to_rank(smem_u32(next_item), r), v, map_to_rank(smem_u32(item_full), r));
           }
+          mbar_expect_tx(smem_u32(item_full), 4);
         }
-        if (tid == 0) mbar_expect_tx(smem_u32(item_full), 4);
+        __syncwarp();
         if (!wait(item_full, (uint32_t)(i - 1))) break;
-        item = (int)*reinterpret_cast<volatile uint32_t*>(next_item);
+        item = (int)lds_volatile(smem_u32(next_item));
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(item_free), 0));
       }
       const int ib = i & 1;
       if (i > 1 && !wait(&info_empty[ib], (uint32_t)((i >> 1) - 1))) break;
       if (item >= p.items) {
-        if (tid == 0) {
+        if (lane == 0) {
           info[ib].row0 = -1;
           mbar_arrive(smem_u32(&info_full[ib]));
         }
@@ -411,110 +410,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       }
       // later tiles first: of a causal sequence these are the long ones
       const int part = item % p.parts, head = (item / p.parts) % p.a.kv_heads;
-      const int row0 = (p.tiles - 1 - item / p.parts / p.a.kv_heads) * 2 * ROWS;
-      // the union of the 256 rows' ranges: thread = rows RPT tid ... RPT tid + RPT - 1
-      constexpr int RPT = 2 * ROWS / (LD_WARPS * 32);
-      int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0, gap = 0, first_lo = -1, last_hi = INT_MAX;
-#pragma unroll
-      for (int h = 0; h < RPT; ++h) {
-        const int r = row0 + RPT * tid + h;
-        if (r < nrows) {
-          const RowKeys rk = row_keys(p.a, r / p.group);
-          if (rk.p_lo < rk.p_hi) {
-            plo = min(plo, rk.p_lo);
-            phi = max(phi, rk.p_hi);
-          }
-          if (rk.k_lo < rk.k_hi) {
-            klo = min(klo, rk.k_lo);
-            khi = max(khi, rk.k_hi);
-          }
-          if (h == 0) first_lo = rk.k_lo;
-          else if (rk.k_lo - last_hi >= KT) gap = 1;
-          last_hi = rk.k_hi;
-        }
-      }
-      const int nx = __shfl_down_sync(0xffffffffu, first_lo, 1);
-      if (lane < 31 && last_hi != INT_MAX && nx >= 0 && nx - last_hi >= KT) gap = 1;
-      const int wfirst = __shfl_sync(0xffffffffu, first_lo, 0), wlast = __shfl_sync(0xffffffffu, last_hi, 31);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        plo = min(plo, __shfl_xor_sync(0xffffffffu, plo, o));
-        phi = max(phi, __shfl_xor_sync(0xffffffffu, phi, o));
-        klo = min(klo, __shfl_xor_sync(0xffffffffu, klo, o));
-        khi = max(khi, __shfl_xor_sync(0xffffffffu, khi, o));
-        gap |= __shfl_xor_sync(0xffffffffu, gap, o);
-      }
-      int* mine = ld_part + (syncs & 1) * LD_WARPS * 7 + lw * 7;
-      if (lane == 0) {
-        mine[0] = plo;
-        mine[1] = phi;
-        mine[2] = klo;
-        mine[3] = khi;
-        mine[4] = gap;
-        mine[5] = wfirst;
-        mine[6] = wlast;
-        mbar_arrive(smem_u32(ldb));
-      }
-      if (!wait(ldb, (uint32_t)syncs)) break;
-      const int* all = ld_part + (syncs & 1) * LD_WARPS * 7;
-      ++syncs;
-#pragma unroll
-      for (int w = 0; w < LD_WARPS; ++w) {
-        plo = min(plo, all[w * 7]);
-        phi = max(phi, all[w * 7 + 1]);
-        klo = min(klo, all[w * 7 + 2]);
-        khi = max(khi, all[w * 7 + 3]);
-        gap |= all[w * 7 + 4];
-        if (w > 0 && all[w * 7 - 1] != INT_MAX && all[w * 7 + 5] >= 0 && all[w * 7 + 5] - all[w * 7 - 1] >= KT)
-          gap = 1;
-      }
-      if (p.counter != nullptr && i > 0 && tid == 0) mbar_arrive_cluster(leader_free);   // all loader threads have read it
-      // this part of the tiles (counted without gaps)
-      const int np = plo < phi ? (phi - plo + KT - 1) / KT : 0, no = klo < khi ? (khi - klo + KT - 1) / KT : 0;
-      const int a0 = (int)((int64_t)(np + no) * part / p.parts), a1 = (int)((int64_t)(np + no) * (part + 1) / p.parts);
+      const int t0 = (p.tiles - 1 - item / p.parts / p.a.kv_heads) * 2 * per, t1 = min(t0 + 2 * per, ntok);
       ItemInfo it;
-      it.row0 = row0;
+      memset(&it, 0, sizeof(it));
+      it.row0 = t0 * p.group;
       it.head = head;
       it.part = part;
-      it.p_lo = a0 < np ? plo + a0 * KT : 0;
-      it.p_hi = a0 < np ? (a1 >= np ? phi : plo + a1 * KT) : 0;
-      it.o_lo = a1 > np ? klo + max(a0 - np, 0) * KT : 0;
-      it.o_hi = a1 > np ? (a1 == np + no ? khi : klo + (a1 - np) * KT) : 0;
-      it.gap = gap;
-      if (tid == 0) {
+      if (t0 < t1) {
+        // the union of the rows' ranges, sequence by sequence: from its first row's first key to its last row's last
+        it.b0 = sequence_by_warp(p.a, t0);
+        it.b1 = sequence_by_warp(p.a, t1 - 1);
+        int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0;
+        unsigned sum = 0;
+        for (int b = it.b0 + lane; b <= it.b1; b += 32) {
+          const int f = max(t0, __ldg(p.a.cu_q + b)), l = min(t1, __ldg(p.a.cu_q + b + 1)) - 1;
+          if (f > l) continue;
+          const RowKeys kf = row_keys_of(p.a, b, f), kl = row_keys_of(p.a, b, l);
+          if (kf.p_lo < kl.p_hi) {
+            plo = min(plo, kf.p_lo);
+            phi = max(phi, kl.p_hi);
+          }
+          if (kf.k_lo < kl.k_hi) {
+            klo = min(klo, kf.k_lo);
+            khi = max(khi, kl.k_hi);
+            sum += (unsigned)(kl.k_hi - kf.k_lo);
+          }
+        }
+        plo = __reduce_min_sync(0xffffffffu, plo);
+        phi = __reduce_max_sync(0xffffffffu, phi);
+        klo = __reduce_min_sync(0xffffffffu, klo);
+        khi = __reduce_max_sync(0xffffffffu, khi);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        // this part of the tiles (counted without gaps)
+        const int np = plo < phi ? (phi - plo + KT - 1) / KT : 0, no = klo < khi ? (khi - klo + KT - 1) / KT : 0;
+        const int a0 = (int)((int64_t)(np + no) * part / p.parts), a1 = (int)((int64_t)(np + no) * (part + 1) / p.parts);
+        it.p_lo = a0 < np ? plo + a0 * KT : 0;
+        it.p_hi = a0 < np ? (a1 >= np ? phi : plo + a1 * KT) : 0;
+        it.o_lo = a1 > np ? klo + max(a0 - np, 0) * KT : 0;
+        it.o_hi = a1 > np ? (a1 == np + no ? khi : klo + (a1 - np) * KT) : 0;
+        it.gap = klo < khi && (unsigned)(khi - klo) - sum >= (unsigned)KT ? 1 : 0;
+      }
+      if (lane == 0) {
         info[ib] = it;
         mbar_arrive(smem_u32(&info_full[ib]));
       }
+      __syncwarp();
       TileIter ti;
       ti.init(p, it);
       int start;
       bool pre;
       if (!ti.next(p, start, pre)) continue;
       if (items > 0 && !wait(q_empty, (uint32_t)(items - 1))) break;
-      // 8 threads copy 128 bytes (64 elements) of a row
-      const int piece = tid & 7;
-      constexpr int RPP = LD_WARPS * 4;          // rows per pass
-#pragma unroll 2
-      for (int j = 0; j < ROWS / RPP; ++j) {
-        const int r = j * RPP + (tid >> 3);
-        const int row = row0 + (int)rank * ROWS + r;
-        const uint32_t dst = smem_u32(smem) + r * 128 + ((piece ^ (r & 7)) << 4);
-        if (row < nrows) {
-          const int t = row / p.group;
-          const uint16_t* src = static_cast<const uint16_t*>(p.a.q) + (int64_t)t * p.a.q_stride +
-                                (int64_t)(head * p.group + row - t * p.group) * p.a.q_head_stride + piece * 8;
+      if (lane == 0) {
+        if (rank == 0) mbar_expect_tx(smem_u32(q_full), (uint32_t)(2 * D * 2 * p.rows));
+        const uint32_t bar = map_to_rank(smem_u32(q_full), 0);
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) cp_async_16(dst + c * 16384, src + c * 64);
-        } else {
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + c * 16384), "r"(0) : "memory");
-        }
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_4d_pair(smem_u32(smem + c * ROWS * 128), &p.tmQ, bar, c * 64, 0, head, t0 + (int)rank * per);
       }
-      cp_async_wait_all();
-      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(leader_q);
       ++items;
     }
   } else {
@@ -542,12 +496,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       it_next = info[ib];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&info_empty[ib]));
-      const int row = it_next.row0 + (int)rank * ROWS + r;
+      const int row = it_next.row0 + (int)rank * p.rows + r;
       rk_next = {0, INT_MAX, 0, INT_MAX};
       tok_next = 0;
-      if (it_next.row0 >= 0 && row < nrows) {
+      if (it_next.row0 >= 0 && r < p.rows && row < nrows) {
         tok_next = row / p.group;
-        rk_next = row_keys(p.a, tok_next);
+        rk_next = row_keys_of(p.a, sequence_of(p.a, tok_next, it_next.b0, it_next.b1 + 1), tok_next);
       }
       return true;
     };
@@ -584,21 +538,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       return true;
     };
     auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & ~1u); };   // as the other side gets it
-    // 32 scores -> weights 2^(c s - mc), their sums, and the packed weights to 16 TMEM columns. seen: bit x for column x
-    auto weights = [&](uint32_t (&s)[32], uint32_t seen, float mc, f32x2 (&sum)[2], uint32_t dst) {
+    // 32 scores -> weights 2^(c s - mc), their sums, and the packed weights to 16 TMEM columns. full: every column is seen, by
+    // every row of the warp; else bit x of seen for column x
+    auto weights = [&](uint32_t (&s)[32], bool full, uint32_t seen, float mc, f32x2 (&sum)[2], uint32_t dst) {
       uint32_t w[16];
-      if (__any_sync(0xffffffffu, seen != 0u)) {
-        const f32x2 nm = x2_pack(-mc, -mc);
-        if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+      const f32x2 nm = x2_pack(-mc, -mc);
+      if (full) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) s[x] = (seen >> x) & 1u ? s[x] : 0xFF800000u;
+        for (int x = 0; x < 32; x += 2) {
+          float e0, e1;
+          const f32x2 y = x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm);
+          x2_unpack(y, e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          w[x / 2] = pack2<BF>(e0, e1);
+          sum[(x / 2) & 1] = x2_add(sum[(x / 2) & 1], x2_pack(e0, e1));
         }
+      } else if (__any_sync(0xffffffffu, seen != 0u)) {
 #pragma unroll
         for (int x = 0; x < 32; x += 2) {
           float e0, e1;
           x2_unpack(x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm), e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
+          e0 = (seen >> x) & 1u ? ex2(e0) : 0.0f;
+          e1 = (seen >> (x + 1)) & 1u ? ex2(e1) : 0.0f;
           w[x / 2] = pack2<BF>(e0, e1);
           sum[(x / 2) & 1] = x2_add(sum[(x / 2) & 1], x2_pack(e0, e1));
         }
@@ -608,16 +570,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       }
       tc_st_32x32b_x16(dst, w);
     };
-    auto chunk_max = [&](const uint32_t (&s)[32], uint32_t seen, float (&mx)[2]) {
-      if (__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+    auto chunk_max = [&](const uint32_t (&s)[32], bool full, uint32_t seen, float (&mx)[2]) {
+      if (full) {
 #pragma unroll
         for (int x = 0; x < 32; x += 4) {
-          mx[0] = max3(mx[0], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
-          mx[1] = max3(mx[1], __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
+          mx[0] = max3_nan(mx[0], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+          mx[1] = max3_nan(mx[1], __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
         }
       } else {
 #pragma unroll
-        for (int x = 0; x < 32; ++x) mx[x & 1] = fmaxf(mx[x & 1], (seen >> x) & 1u ? __uint_as_float(s[x]) : -INFINITY);
+        for (int x = 0; x < 32; ++x) mx[x & 1] = max_nan(mx[x & 1], (seen >> x) & 1u ? __uint_as_float(s[x]) : -INFINITY);
       }
     };
 
@@ -627,31 +589,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       rk = rk_next;
       tok = tok_next;
       if (it.row0 < 0) break;
-      const int row = it.row0 + (int)rank * ROWS + r;
-      const bool live = row < nrows;
+      const int row = it.row0 + (int)rank * p.rows + r;
+      const bool live = r < p.rows && row < nrows;
       const bool any_live = __any_sync(0xffffffffu, live);
       const bool none = rk.p_lo >= rk.p_hi && rk.k_lo >= rk.k_hi;
       float m = -INFINITY, l = 0.0f;             // the maximum in use (of scores times c), the sum of this half's weights
       TileIter ti;
       ti.init(p, it);
       int j = 0;
-      // a tile: which of this thread's 64 columns its row sees, and whether any row of the warp sees any of the 128
-      struct Tile { uint32_t seen0, seen1; bool some; } cur;
+      // what the warp's rows see of the prefix and of their own keys: all of them [f_lo, f_hi), none anything outside [s_lo, s_hi)
+      struct Range { int f_lo, f_hi, s_lo, s_hi; };
+      auto range = [&](int lo, int hi) {
+        const bool e = lo >= hi;
+        return Range{__reduce_max_sync(0xffffffffu, lo), __reduce_min_sync(0xffffffffu, hi),
+                     __reduce_min_sync(0xffffffffu, e ? INT_MAX : lo), __reduce_max_sync(0xffffffffu, e ? 0 : hi)};
+      };
+      // keys from the part's end on are the next part's, whose first tile may begin inside this one where there are gaps
+      const int p_hi = min(rk.p_hi, it.p_hi), k_hi = min(rk.k_hi, it.o_hi);
+      const Range pr = range(rk.p_lo, p_hi), kr = range(rk.k_lo, k_hi);
+      struct Tile {
+        bool full, some;                         // all rows of the warp see all 128 keys; some row sees some key
+        uint32_t seen0, seen1;                   // if not full: which of this thread's 64 columns its row sees
+      } cur;
       auto next = [&](Tile& t) {
         int start;
         bool pre;
         if (!ti.next(p, start, pre)) return false;
-        // keys from the part's end on are the next part's, whose first tile may begin inside this one where there are gaps
-        const int lo = pre ? rk.p_lo : rk.k_lo, hi = pre ? min(rk.p_hi, it.p_hi) : min(rk.k_hi, it.o_hi);
-        const int a0 = max(lo - start, 0), a1 = hi - start;          // columns [a0, a1) are seen
-        auto seen = [&](int col) {                                   // of columns col .. col + 31
-          const int f = min(max(a0 - col, 0), 32), e = min(max(a1 - col, 0), 32);
-          const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_f = f == 32 ? 0xffffffffu : (1u << f) - 1u;
-          return below_e & ~below_f;
-        };
-        t.seen0 = seen(half * 64);
-        t.seen1 = seen(half * 64 + 32);
-        t.some = __any_sync(0xffffffffu, a0 < KT && a1 > a0);
+        t.full = pre ? start >= pr.f_lo && start + KT <= pr.f_hi : start >= kr.f_lo && start + KT <= kr.f_hi;
+        t.some = pre ? start < pr.s_hi && start + KT > pr.s_lo : start < kr.s_hi && start + KT > kr.s_lo;
+        if (!t.full) {
+          const int a0 = (pre ? rk.p_lo : rk.k_lo) - start, a1 = (pre ? p_hi : k_hi) - start;   // columns [a0, a1) are seen
+          auto seen = [&](int col) {                                   // of columns col .. col + 31
+            const int f = min(max(a0 - col, 0), 32), e = min(max(a1 - col, 0), 32);
+            const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_f = f == 32 ? 0xffffffffu : (1u << f) - 1u;
+            return below_e & ~below_f;
+          };
+          t.seen0 = seen(half * 64);
+          t.seen1 = seen(half * 64 + 32);
+        }
         return true;
       };
       uint32_t s0[32], s1[32];
@@ -666,16 +641,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         tc_wait_ld(x0);
         loaded(x1);
         float mx[2] = {-INFINITY, -INFINITY};
-        chunk_max(x0, t.seen0, mx);
-        chunk_max(x1, t.seen1, mx);
-        mine = cut(fmaxf(mx[0], mx[1]));
+        chunk_max(x0, t.full, t.seen0, mx);
+        chunk_max(x1, t.full, t.seen1, mx);
+        mine = cut(max_nan(mx[0], mx[1]));
         post(mine);
       };
       // the softmax of one tile whose scores are in registers and whose half maxima are posted
       auto weigh = [&](const Tile& t, uint32_t (&x0)[32], uint32_t (&x1)[32]) {
         float top;
         if (!receive(top)) return false;
-        top = fmaxf(top, mine) * c;
+        top = max_nan(top, mine) * c;
+        if (!(top < INFINITY)) l = NAN;          // a score that is NaN or infinite: so are the row's weights
         const bool grow = top - m > THR;         // from -inf on the first key
         const bool rescale = grow && m != -INFINITY;
         if (__any_sync(0xffffffffu, rescale)) {
@@ -698,8 +674,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         const float mc = (m == -INFINITY ? 0.0f : m) - SHIFT;
         f32x2 sum[2] = {0ull, 0ull};
         // P takes the place of the first 64 columns of S, which both halves have read
-        weights(x0, t.seen0, mc, sum, scol(g) + half * 32);
-        weights(x1, t.seen1, mc, sum, scol(g) + half * 32 + 16);
+        weights(x0, t.full, t.seen0, mc, sum, scol(g) + half * 32);
+        weights(x1, t.full, t.seen1, mc, sum, scol(g) + half * 32 + 16);
         float y0, y1;
         x2_unpack(x2_add(sum[0], sum[1]), y0, y1);
         l += y0 + y1;
@@ -722,7 +698,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         ++g;
         ++j;
       };
-      while (next(cur)) {
+      bool more = next(cur);
+      while (more) {
         if (!(ok = wait(&s_full[g % NB], (uint32_t)(g / NB)))) break;
         if (any_live) {
           if (cur.some) {
@@ -734,6 +711,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           }
         }
         done();
+        more = next(cur);
       }
       if (!ok) break;
       if (!(ok = fetch(i + 1))) break;           // while the last products run
@@ -747,7 +725,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         tc_fence_after();
         constexpr int HC = D / 2;
         const int head = it.head * p.group + (row - tok * p.group);
-        const int64_t part_row = ((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * ROWS) + row;
+        const int64_t part_row = ((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * p.rows) + row;
         const float inv = none ? 0.0f : 1.0f / l;
         const f32x2 inv2 = x2_pack(inv, inv);
         uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride + half * HC;
@@ -845,7 +823,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   const int tok = (int)(id / p.a.q_heads), head = (int)(id - (int64_t)tok * p.a.q_heads);
   if ((int64_t)tok * p.group >= row_count(p)) return;
   const int kvh = head / p.group;
-  const int64_t stride = (int64_t)p.tiles * 2 * ROWS;
+  const int64_t stride = (int64_t)p.tiles * 2 * p.rows;
   const int64_t first = (int64_t)kvh * stride + (int64_t)tok * p.group + (head - kvh * p.group);
   float m = -INFINITY;
   for (int s = 0; s < p.parts; ++s) m = fmaxf(m, p.part_ml[first + (int64_t)s * p.a.kv_heads * stride].x);
@@ -901,7 +879,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
 
 // Row tiles, parts of the keys, and the workspace: counter, partial maxima and sums, partial outputs.
 struct Plan {
-  int group, tiles, parts, items, pairs;
+  int group, rows, tiles, parts, items, pairs;
   size_t ml, o, total;
 };
 
@@ -909,7 +887,8 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   Plan pl;
   pl.group = a.q_heads / a.kv_heads;
   const int64_t rows = a.q_tokens * pl.group;
-  pl.tiles = (int)ceil_div64(rows, 2 * ROWS);
+  pl.rows = ROWS / pl.group * pl.group;
+  pl.tiles = (int)ceil_div64(rows, 2 * pl.rows);
   const int64_t base = (int64_t)pl.tiles * a.kv_heads;
   const int pairs = num_sms / 2 > 0 ? num_sms / 2 : 1;
   const int64_t keys = a.prefix + a.k_tokens;
@@ -922,7 +901,7 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   pl.items = (int)items;
   pl.pairs = (int)(items < pairs ? items : pairs);
   pl.ml = 256;
-  const size_t prow = pl.parts > 1 ? (size_t)pl.parts * a.kv_heads * pl.tiles * 2 * ROWS : 0;
+  const size_t prow = pl.parts > 1 ? (size_t)pl.parts * a.kv_heads * pl.tiles * 2 * pl.rows : 0;
   pl.o = pl.ml + ((prow * 8 + 255) & ~size_t(255));
   pl.total = pl.o + prow * a.head_dim * 4;
   return pl;
@@ -935,6 +914,7 @@ static int launch_t(const AttentionLaunch& l, const Plan& pl, cudaStream_t s) {
   memset(&p, 0, sizeof(p));
   p.a = a;
   p.group = pl.group;
+  p.rows = pl.rows;
   p.tiles = pl.tiles;
   p.parts = pl.parts;
   p.items = pl.items;
@@ -945,6 +925,8 @@ static int launch_t(const AttentionLaunch& l, const Plan& pl, cudaStream_t s) {
   p.part_o = reinterpret_cast<float*>(ws + pl.o);
   p.timeout_ns = l.timeout_ns;
   constexpr int VB = D == 64 ? 32 : 64;
+  if (make_map_rows(&p.tmQ, a.q, a.q_tokens, a.q_stride, a.kv_heads, pl.group, a.q_head_stride, D, pl.rows / pl.group))
+    return REAXMOE_ERR_CUDA;
   if (a.k_tokens > 0 &&
       (make_map_heads(&p.tmK, a.k, a.k_tokens, a.k_stride, a.kv_heads, a.k_head_stride, D, 64, 64) ||
        make_map_heads(&p.tmV, a.v, a.k_tokens, a.v_stride, a.kv_heads, a.v_head_stride, D, VB, KT)))

@@ -17,12 +17,25 @@ struct RowKeys {
   int k_lo, k_hi;   // keys of the packed k / v seen (row numbers of the packed tensors)
 };
 
-// the last b with cu_q[b] <= t (sequences of no rows are passed over); t < cu_q[seqs]
-__device__ __forceinline__ int sequence_of(const reaxmoe_attention_args& a, int t) {
-  int b0 = 0, b1 = a.seqs;
+// the last b of [b0, b1) with cu_q[b] <= t (sequences of no rows are passed over); t < cu_q[b1]
+__device__ __forceinline__ int sequence_of(const reaxmoe_attention_args& a, int t, int b0, int b1) {
   while (b1 - b0 > 1) {
     const int mid = (b0 + b1) >> 1;
     if (__ldg(a.cu_q + mid) <= t) b0 = mid; else b1 = mid;
+  }
+  return b0;
+}
+
+// the same of all sequences by a whole warp, 32 at a time
+__device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a, int t) {
+  const int lane = threadIdx.x & 31;
+  int b0 = 0, len = a.seqs;
+  while (len > 1) {
+    const int step = (len + 31) / 32, i = lane * step;
+    const bool le = i < len && __ldg(a.cu_q + b0 + i) <= t;
+    const int c = max(__popc(__ballot_sync(0xffffffffu, le)), 1) - 1;
+    b0 += min(c * step, len - 1);
+    len = max(min(step, len - c * step), 1);
   }
   return b0;
 }
@@ -47,7 +60,7 @@ __device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, 
   return r;
 }
 __device__ __forceinline__ RowKeys row_keys(const reaxmoe_attention_args& a, int t) {
-  return row_keys_of(a, sequence_of(a, t), t);
+  return row_keys_of(a, sequence_of(a, t, 0, a.seqs), t);
 }
 
 template <bool BF>

@@ -54,6 +54,14 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
 // D[256 x N] (+)= A[256 x 16] B[N x 16]^T over the CTA pair: each CTA holds its own 128 rows of A and D and half of B's N rows
 __device__ __forceinline__ void mma_pair_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -144,9 +152,15 @@ __device__ __forceinline__ f32x2 x2_mul(f32x2 a, f32x2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// maxima that are NaN when an operand is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -179,6 +193,23 @@ inline int make_map_heads(CUtensorMap* tm, const void* base, int64_t tokens, int
   const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, box_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : REAXMOE_ERR_CUDA;
+}
+
+// [tokens, kv_heads, group, dim]: box [box_tokens, 1, group, 64], whose 128-byte rows are the (token, head of the group) pairs
+inline int make_map_rows(CUtensorMap* tm, const void* base, int64_t tokens, int64_t token_stride, int kv_heads, int group,
+                         int64_t head_stride, int dim, int box_tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return REAXMOE_ERR_CUDA;
+  if (kv_heads * group == 1) head_stride = dim;
+  if (tokens == 1) token_stride = (int64_t)head_stride * kv_heads * group;
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)group, (cuuint64_t)kv_heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[3] = {(cuuint64_t)head_stride * 2, (cuuint64_t)head_stride * group * 2, (cuuint64_t)token_stride * 2};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)group, 1u, (cuuint32_t)box_tokens};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : REAXMOE_ERR_CUDA;
 }
 

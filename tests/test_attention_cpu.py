@@ -29,6 +29,7 @@ def test_a_good_call_needs_its_workspace():
 
 @pytest.mark.parametrize("kw,code", [
     (dict(head_dim=96), L.ERR_BAD_SHAPE), (dict(q_heads=12, kv_heads=8), L.ERR_BAD_SHAPE), (dict(kv_heads=0), L.ERR_BAD_SHAPE),
+    (dict(q_heads=129, kv_heads=1), L.ERR_BAD_SHAPE),
     (dict(seqs=-1), L.ERR_BAD_SHAPE), (dict(q_tokens=-1), L.ERR_BAD_SHAPE), (dict(k_tokens=1 << 31), L.ERR_BAD_SHAPE),
     (dict(k_tokens=1 << 30, prefix=1 << 30), L.ERR_BAD_SHAPE), (dict(q_tokens=(1 << 31) - 70000), L.ERR_BAD_SHAPE),
     (dict(prefix=-5), L.ERR_BAD_SHAPE), (dict(dtype=2), L.ERR_UNSUPPORTED), (dict(causal=2), L.ERR_BAD_SHAPE),

@@ -97,7 +97,7 @@ def test_prompts(d, dtype, lens):
     run(lens, d=d, dtype=dtype, seed=sum(lens))
 
 
-@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 8), (6, 2), (5, 1), (14, 2), (16, 1)])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (8, 8), (6, 2), (5, 1), (14, 2), (16, 1), (96, 2), (128, 1), (77, 1)])
 def test_groups_of_heads(hq, hk):
     run((70, 3, 61), hq=hq, hk=hk, d=128, seed=hq)
 
