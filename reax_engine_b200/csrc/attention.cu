@@ -90,7 +90,7 @@ struct TileIter {
   int pc, ph, oc, oh;
   int b, b_end, t0, t1, lo, hi;
   bool gap;
-  __device__ __forceinline__ void need(const reaxmoe_attention_args& a) {
+  __device__ __noinline__ void need(const reaxmoe_attention_args& a) {
     const int q0 = __ldg(a.cu_q + b), q1 = __ldg(a.cu_q + b + 1);
     const int f = max(t0, q0), l = min(t1, q1) - 1;
     lo = 0;
@@ -123,6 +123,7 @@ struct TileIter {
     }
     pre = false;
     if (gap) {
+#pragma unroll 1
       while (hi <= oc) {
         if (b >= b_end) return false;
         ++b;
@@ -136,6 +137,11 @@ struct TileIter {
     return true;
   }
 };
+
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                        unsigned long long timeout_ns) {
+  return wait_bounded(bar, parity, abort_flag, status, timeout_ns);
+}
 
 // MN-major V tile: 128-byte swizzle with 64-dim blocks 16 KiB apart (LBO) and 8-key groups 1024 bytes apart (SBO); for D = 64 a
 // CTA's half is 32 dims wide: 64-byte swizzle, 8-key groups 512 bytes apart.
@@ -184,13 +190,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     set_status(p.a.status, REAXMOE_ERR_UNSUPPORTED);
     return;
   }
+  // a bounded wait; what is not there at once is waited for out of line (the kernel's code has to stay in the instruction cache)
   auto wait1 = [&](uint64_t* bar, uint32_t parity) {
-    return wait_bounded(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns);
+    return mbar_try_wait(smem_u32(bar), parity & 1u) || wait_longer(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns);
   };
   // every lane of a warp waits and all get the same answer
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, wait_bounded(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns)) != 0;
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait1(bar, parity)) != 0; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
@@ -278,6 +283,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       }
       // let the last loads land before the CTA may exit (only matters after an abort)
       if (rank == 0)
+#pragma unroll 1
         for (int f = n - 1; f >= 0 && f >= n - NS; --f) wait_drain(smem_u32(&full[f % NS]), (uint32_t)(f / NS) & 1u);
     }
   } else if (warp == 9) {
@@ -422,6 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         it.b1 = sequence_by_warp(p.a, t1 - 1);
         int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0;
         unsigned sum = 0;
+#pragma unroll 1
         for (int b = it.b0 + lane; b <= it.b1; b += 32) {
           const int f = max(t0, __ldg(p.a.cu_q + b)), l = min(t1, __ldg(p.a.cu_q + b + 1)) - 1;
           if (f > l) continue;
@@ -443,7 +450,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         sum = __reduce_add_sync(0xffffffffu, sum);
         // this part of the tiles (counted without gaps)
         const int np = plo < phi ? (phi - plo + KT - 1) / KT : 0, no = klo < khi ? (khi - klo + KT - 1) / KT : 0;
-        const int a0 = (int)((int64_t)(np + no) * part / p.parts), a1 = (int)((int64_t)(np + no) * (part + 1) / p.parts);
+        // (tiles times parts fits: at most 2^24 tiles, and parts only where the items are fewer than the pairs)
+        const int a0 = (int)((unsigned)(np + no) * (unsigned)part / (unsigned)p.parts);
+        const int a1 = (int)((unsigned)(np + no) * (unsigned)(part + 1) / (unsigned)p.parts);
         it.p_lo = a0 < np ? plo + a0 * KT : 0;
         it.p_hi = a0 < np ? (a1 >= np ? phi : plo + a1 * KT) : 0;
         it.o_lo = a1 > np ? klo + max(a0 - np, 0) * KT : 0;
@@ -522,6 +531,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       ++x_n;
       uint32_t v = lds_volatile(at);
       uint64_t t0 = 0;
+#pragma unroll 1
       for (uint32_t n = 1; !__all_sync(0xffffffffu, (v & 1u) == tag); ++n) {
         if ((n & 63u) == 0u) {
           if (t0 == 0) t0 = globaltimer();
@@ -538,29 +548,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       return true;
     };
     auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & ~1u); };   // as the other side gets it
-    // 32 scores -> weights 2^(c s - mc), their sums, and the packed weights to 16 TMEM columns. full: every column is seen, by
-    // every row of the warp; else bit x of seen for column x
-    auto weights = [&](uint32_t (&s)[32], bool full, uint32_t seen, float mc, f32x2 (&sum)[2], uint32_t dst) {
+    // 32 scores -> weights 2^(c s - mc), their sums, and the packed weights to 16 TMEM columns; any: some row of the warp sees
+    // some of the columns
+    auto weights = [&](const uint32_t (&s)[32], bool any, float mc, f32x2 (&sum)[2], uint32_t dst) {
       uint32_t w[16];
-      const f32x2 nm = x2_pack(-mc, -mc);
-      if (full) {
-#pragma unroll
-        for (int x = 0; x < 32; x += 2) {
-          float e0, e1;
-          const f32x2 y = x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm);
-          x2_unpack(y, e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          w[x / 2] = pack2<BF>(e0, e1);
-          sum[(x / 2) & 1] = x2_add(sum[(x / 2) & 1], x2_pack(e0, e1));
-        }
-      } else if (__any_sync(0xffffffffu, seen != 0u)) {
+      if (any) {
+        const f32x2 nm = x2_pack(-mc, -mc);
 #pragma unroll
         for (int x = 0; x < 32; x += 2) {
           float e0, e1;
           x2_unpack(x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm), e0, e1);
-          e0 = (seen >> x) & 1u ? ex2(e0) : 0.0f;
-          e1 = (seen >> (x + 1)) & 1u ? ex2(e1) : 0.0f;
+          e0 = ex2(e0);
+          e1 = ex2(e1);
           w[x / 2] = pack2<BF>(e0, e1);
           sum[(x / 2) & 1] = x2_add(sum[(x / 2) & 1], x2_pack(e0, e1));
         }
@@ -570,17 +569,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       }
       tc_st_32x32b_x16(dst, w);
     };
-    auto chunk_max = [&](const uint32_t (&s)[32], bool full, uint32_t seen, float (&mx)[2]) {
-      if (full) {
+    auto hide = [&](uint32_t (&s)[32], uint32_t seen) {          // scores that the row does not see: weight 0
 #pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          mx[0] = max3_nan(mx[0], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
-          mx[1] = max3_nan(mx[1], __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < 32; ++x) mx[x & 1] = max_nan(mx[x & 1], (seen >> x) & 1u ? __uint_as_float(s[x]) : -INFINITY);
-      }
+      for (int x = 0; x < 32; ++x) s[x] = (seen >> x) & 1u ? s[x] : 0xFF800000u;
     };
 
     if (!fetch(0)) ok = false;
@@ -609,6 +600,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       const Range pr = range(rk.p_lo, p_hi), kr = range(rk.k_lo, k_hi);
       struct Tile {
         bool full, some;                         // all rows of the warp see all 128 keys; some row sees some key
+        bool any0, any1;                         // some row sees some of this thread's first / last 32 columns
         uint32_t seen0, seen1;                   // if not full: which of this thread's 64 columns its row sees
       } cur;
       auto next = [&](Tile& t) {
@@ -617,6 +609,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         if (!ti.next(p, start, pre)) return false;
         t.full = pre ? start >= pr.f_lo && start + KT <= pr.f_hi : start >= kr.f_lo && start + KT <= kr.f_hi;
         t.some = pre ? start < pr.s_hi && start + KT > pr.s_lo : start < kr.s_hi && start + KT > kr.s_lo;
+        t.any0 = t.any1 = true;
         if (!t.full) {
           const int a0 = (pre ? rk.p_lo : rk.k_lo) - start, a1 = (pre ? p_hi : k_hi) - start;   // columns [a0, a1) are seen
           auto seen = [&](int col) {                                   // of columns col .. col + 31
@@ -626,6 +619,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           };
           t.seen0 = seen(half * 64);
           t.seen1 = seen(half * 64 + 32);
+          t.any0 = __any_sync(0xffffffffu, t.seen0 != 0u);
+          t.any1 = __any_sync(0xffffffffu, t.seen1 != 0u);
         }
         return true;
       };
@@ -640,9 +635,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       auto find_max = [&](const Tile& t, uint32_t (&x0)[32], uint32_t (&x1)[32]) {
         tc_wait_ld(x0);
         loaded(x1);
+        if (!t.full) {
+          hide(x0, t.seen0);
+          hide(x1, t.seen1);
+        }
         float mx[2] = {-INFINITY, -INFINITY};
-        chunk_max(x0, t.full, t.seen0, mx);
-        chunk_max(x1, t.full, t.seen1, mx);
+#pragma unroll
+        for (int x = 0; x < 32; x += 2) {
+          mx[0] = max3_nan(mx[0], __uint_as_float(x0[x]), __uint_as_float(x0[x + 1]));
+          mx[1] = max3_nan(mx[1], __uint_as_float(x1[x]), __uint_as_float(x1[x + 1]));
+        }
         mine = cut(max_nan(mx[0], mx[1]));
         post(mine);
       };
@@ -674,8 +676,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         const float mc = (m == -INFINITY ? 0.0f : m) - SHIFT;
         f32x2 sum[2] = {0ull, 0ull};
         // P takes the place of the first 64 columns of S, which both halves have read
-        weights(x0, t.full, t.seen0, mc, sum, scol(g) + half * 32);
-        weights(x1, t.full, t.seen1, mc, sum, scol(g) + half * 32 + 16);
+        weights(x0, t.any0, mc, sum, scol(g) + half * 32);
+        weights(x1, t.any1, mc, sum, scol(g) + half * 32 + 16);
         float y0, y1;
         x2_unpack(x2_add(sum[0], sum[1]), y0, y1);
         l += y0 + y1;
@@ -699,6 +701,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         ++j;
       };
       bool more = next(cur);
+#pragma unroll 1
       while (more) {
         if (!(ok = wait(&s_full[g % NB], (uint32_t)(g / NB)))) break;
         if (any_live) {
@@ -730,7 +733,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         const f32x2 inv2 = x2_pack(inv, inv);
         uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride + half * HC;
         f32x2 check = 0ull;                      // becomes NaN with the first value that is not finite
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < HC; x += 32) {
           uint32_t o[32];
           if (j > 0) {
@@ -789,6 +792,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
             if (live && p.a.lse != nullptr)
               p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
             uint32_t again = mine | flags[4 + quarter];
+#pragma unroll 1
             while (again != 0u) {
               const int src = __ffs(again) - 1;
               again &= again - 1u;
@@ -818,10 +822,10 @@ template <int D, bool BF>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
   constexpr float SHIFT = BF ? 0.0f : 12.0f;
   constexpr int W = D / 32;
-  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int id = (int)(blockIdx.x * 8 + (threadIdx.x >> 5));     // fits: the rows of fewer tiles than there are pairs
   const int lane = threadIdx.x & 31;
-  const int tok = (int)(id / p.a.q_heads), head = (int)(id - (int64_t)tok * p.a.q_heads);
-  if ((int64_t)tok * p.group >= row_count(p)) return;
+  const int tok = id / p.a.q_heads, head = id - tok * p.a.q_heads;
+  if (tok * p.group >= row_count(p)) return;
   const int kvh = head / p.group;
   const int64_t stride = (int64_t)p.tiles * 2 * p.rows;
   const int64_t first = (int64_t)kvh * stride + (int64_t)tok * p.group + (head - kvh * p.group);

@@ -18,7 +18,8 @@ struct RowKeys {
 };
 
 // the last b of [b0, b1) with cu_q[b] <= t (sequences of no rows are passed over); t < cu_q[b1]
-__device__ __forceinline__ int sequence_of(const reaxmoe_attention_args& a, int t, int b0, int b1) {
+__device__ __noinline__ int sequence_of(const reaxmoe_attention_args& a, int t, int b0, int b1) {
+#pragma unroll 1
   while (b1 - b0 > 1) {
     const int mid = (b0 + b1) >> 1;
     if (__ldg(a.cu_q + mid) <= t) b0 = mid; else b1 = mid;
@@ -30,6 +31,7 @@ __device__ __forceinline__ int sequence_of(const reaxmoe_attention_args& a, int 
 __device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a, int t) {
   const int lane = threadIdx.x & 31;
   int b0 = 0, len = a.seqs;
+#pragma unroll 1
   while (len > 1) {
     const int step = (len + 31) / 32, i = lane * step;
     const bool le = i < len && __ldg(a.cu_q + b0 + i) <= t;
@@ -42,7 +44,7 @@ __device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a,
 
 // Keys that query token t of sequence b sees. The cumulative lengths are cut to the tensors, so that no value of theirs makes
 // a later access leave them.
-__device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
+__device__ __noinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
   const int kt = (int)a.k_tokens, P = (int)a.prefix;
   const int ks = min(max(__ldg(a.cu_k + b), 0), kt);
   const int n = min(max(__ldg(a.cu_k + b + 1), ks), kt) - ks;
@@ -99,6 +101,7 @@ __device__ __noinline__ void row_by_warp(const reaxmoe_attention_args& a, int t,
   const float c = a.scale * 1.4426950408889634f;  // scores in units of log2
   float m = -INFINITY, l = 0.0f;
   auto keys = [&](const void* kb, int64_t ks, int64_t khs, const void* vb, int64_t vs, int64_t vhs, int lo, int hi) {
+#pragma unroll 1
     for (int j = lo; j < hi; ++j) {
       float2 k[W], v[W];
       load(kb, j, ks, khs, kvh, k);
