@@ -25,6 +25,7 @@
 //   warp 8        K / V producer: ring of slots, alternately half a K tile (64 keys x D) and half a V tile (128 keys x D / 2)
 //   warp 9        allocates TMEM; in the leader CTA one thread issues all MMAs of the pair
 //   warp 10       loader: takes the next item, works out its key ranges, loads its Q rows (TMA)
+//   warps 12..15  output: O from TMEM, divided by the sums, while the softmax warps are at the next item's first tiles
 // Items (row tile, KV head, part of the keys) are taken in order, the first by pair number, further ones from a counter.
 // With few rows an item's keys are split over several pairs, which leave partial sums that combine_kernel joins.
 // All waits are bounded (globaltimer); a timeout records REAXMOE_ERR_DEVICE_TIMEOUT and the CTA winds down.
@@ -40,7 +41,11 @@ namespace attn {
 constexpr int ROWS = 128;                 // query rows per CTA
 constexpr int KT = 128;                   // keys per tile
 constexpr int SM_WARPS = 8;               // softmax warps
-constexpr int THREADS = (SM_WARPS + 3) * 32;
+constexpr int OUT_WARP0 = 12, OUT_WARPS = 4;
+constexpr int THREADS = (OUT_WARP0 + OUT_WARPS) * 32;
+// registers a thread: the kernel is launched with 128 x 512 of them, and the warp groups share these out (the sum stays 512)
+constexpr int REGS_SOFTMAX = 168, REGS_CONTROL = 64, REGS_OUT = 112;
+static_assert(2 * REGS_SOFTMAX + REGS_CONTROL + REGS_OUT == 4 * 128 && THREADS == 512, "register shares");
 
 template <int D>
 struct Layout {
@@ -90,7 +95,7 @@ struct TileIter {
   int pc, ph, oc, oh;
   int b, b_end, t0, t1, lo, hi;
   bool gap;
-  __device__ __noinline__ void need(const reaxmoe_attention_args& a) {
+  __device__ __forceinline__ void need(const reaxmoe_attention_args& a) {
     const int q0 = __ldg(a.cu_q + b), q1 = __ldg(a.cu_q + b + 1);
     const int f = max(t0, q0), l = min(t1, q1) - 1;
     lo = 0;
@@ -138,11 +143,6 @@ struct TileIter {
   }
 };
 
-__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                        unsigned long long timeout_ns) {
-  return wait_bounded(bar, parity, abort_flag, status, timeout_ns);
-}
-
 // MN-major V tile: 128-byte swizzle with 64-dim blocks 16 KiB apart (LBO) and 8-key groups 1024 bytes apart (SBO); for D = 64 a
 // CTA's half is 32 dims wide: 64-byte swizzle, 8-key groups 512 bytes apart.
 template <int D>
@@ -168,18 +168,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   uint64_t* p_full = s_full + NB;      // [NB] (leader's) P is in TMEM (16 warps of the pair)
   uint64_t* pv_done = p_full + NB;     // [2] a tile's P V is in O (commit to both)
   uint64_t* o_full = pv_done + 2;      // the item's O is complete (commit to both)
-  uint64_t* o_empty = o_full + 1;      // (leader's) O has been read out (16 warps)
+  uint64_t* o_empty = o_full + 1;      // (leader's) O has been read out (8 warps of the pair)
   uint64_t* q_full = o_empty + 1;      // (leader's) both CTAs' Q rows landed (tx)
   uint64_t* q_empty = q_full + 1;      // the item's Q K^T are done (commit to both)
   uint64_t* info_full = q_empty + 1;   // [2] item info is there
-  uint64_t* info_empty = info_full + 2;// [2] item info has been read (producer, MMA, 8 softmax warps)
+  uint64_t* info_empty = info_full + 2;// [2] item info has been read (producer, MMA, softmax and output warps)
   uint64_t* item_full = info_empty + 2;// the next item's number arrived (tx)
   uint64_t* item_free = item_full + 1; // (leader's) both CTAs took it
-  uint64_t* xb = item_free + 1;        // [4] the two warps of a lane quarter exchange sums and flags
-  uint64_t* drainb = xb + 4;
-  ItemInfo* info = reinterpret_cast<ItemInfo*>(smem + L::bars + 512);   // [2]
-  uint32_t* flags = reinterpret_cast<uint32_t*>(info + 2);              // [2][4] rows to be done again
-  uint32_t* next_item = flags + 8;
+  uint64_t* l_full = item_free + 1;    // the item's factors 1 / sum are in shared memory (4 softmax warps)
+  uint64_t* l_empty = l_full + 1;      // they have been read (4 output warps)
+  uint64_t* drainb = l_empty + 1;
+  float* inv_l = reinterpret_cast<float*>(drainb + 1);                  // [ROWS]
+  ItemInfo* info = reinterpret_cast<ItemInfo*>(inv_l + ROWS);           // [2]
+  uint32_t* next_item = reinterpret_cast<uint32_t*>(info + 2);
   uint32_t* tmem_holder = next_item + 1;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
@@ -190,9 +191,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     set_status(p.a.status, REAXMOE_ERR_UNSUPPORTED);
     return;
   }
-  // a bounded wait; what is not there at once is waited for out of line (the kernel's code has to stay in the instruction cache)
   auto wait1 = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_try_wait(smem_u32(bar), parity & 1u) || wait_longer(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns);
+    return wait_bounded(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns);
   };
   // every lane of a warp waits and all get the same answer
   auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait1(bar, parity)) != 0; };
@@ -209,15 +209,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&pv_done[b]), 1);
       mbar_init(smem_u32(&info_full[b]), 1);
-      mbar_init(smem_u32(&info_empty[b]), SM_WARPS + 2);
+      mbar_init(smem_u32(&info_empty[b]), SM_WARPS + OUT_WARPS + 2);
     }
     mbar_init(smem_u32(o_full), 1);
-    mbar_init(smem_u32(o_empty), 2 * SM_WARPS);
+    mbar_init(smem_u32(o_empty), 2 * OUT_WARPS);
     mbar_init(smem_u32(q_full), 1);
     mbar_init(smem_u32(q_empty), 1);
     mbar_init(smem_u32(item_full), 1);
     mbar_init(smem_u32(item_free), 2);
-    for (int b = 0; b < 4; ++b) mbar_init(smem_u32(&xb[b]), 2);
+    mbar_init(smem_u32(l_full), SM_WARPS / 2);
+    mbar_init(smem_u32(l_empty), OUT_WARPS);
     mbar_init(smem_u32(drainb), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -233,6 +234,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
 
+  if (warp >= SM_WARPS && warp < OUT_WARP0) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
   if (warp == 8) {
     // ------------------------------------------------------------------------------------------ K / V producer
     if (elect_one()) {
@@ -480,8 +483,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       __syncwarp();
       ++items;
     }
-  } else {
-    // ------------------------------------------------------------------------------------------ softmax, output
+  }
+  } else if (warp < SM_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    // ------------------------------------------------------------------------------------------ softmax
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -489,10 +494,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     const int nrows = row_count(p);
     const float c = p.a.scale * 1.4426950408889634f;
     const f32x2 c2 = x2_pack(c, c);
-    const uint32_t p_full0 = map_to_rank(smem_u32(&p_full[0]), 0), leader_o = map_to_rank(smem_u32(o_empty), 0);
+    const uint32_t p_full0 = map_to_rank(smem_u32(&p_full[0]), 0);
     const uint32_t x_mine = smem_u32(smem + L::words) + (uint32_t)(half * ROWS + r) * 4;
     const uint32_t x_other = smem_u32(smem + L::words) + (uint32_t)((half ^ 1) * ROWS + r) * 4;
-    int g = 0, items = 0, ex = 0, x_n = 0;
+    int g = 0, x_n = 0;
     bool ok = true;
 
     ItemInfo it, it_next;
@@ -513,12 +518,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         rk_next = row_keys_of(p.a, sequence_of(p.a, tok_next, it_next.b0, it_next.b1 + 1), tok_next);
       }
       return true;
-    };
-    // both warps of a lane quarter meet: what each wrote to shared memory before is there for the other afterwards
-    auto meet = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&xb[quarter]));
-      return wait(&xb[quarter], (uint32_t)ex++);
     };
     // The halves of a row exchange a value (maximum, sum) through one word each, whose lowest bit says which use of the word it
     // is: a word is used every other time, and written again only after the other side has gone on to the next one. Both
@@ -717,39 +716,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         more = next(cur);
       }
       if (!ok) break;
-      if (!(ok = fetch(i + 1))) break;           // while the last products run
-      // the item's rows: o = O / l, or the partial sums of this part
+      // the sums, for the output warps
       if (any_live) {
         float other;
         post(l);
         if (!(ok = receive(other))) break;
         l = cut(l) + other;
-        if (j > 0 && !(ok = wait(o_full, (uint32_t)items))) break;
+      }
+      if (half == 0) {
+        if (i > 0 && !(ok = wait(l_empty, (uint32_t)(i - 1)))) break;
+        inv_l[r] = none ? 0.0f : 1.0f / l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(l_full));
+        if (live) {
+          const int in_group = row - tok * p.group;
+          if (p.parts > 1)
+            p.part_ml[((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * p.rows) + row] = make_float2(m, l);
+          else if (p.a.lse != nullptr)
+            p.a.lse[(int64_t)tok * p.a.q_heads + it.head * p.group + in_group] =
+                none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
+        }
+      }
+      if (!(ok = fetch(i + 1))) break;
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OUT));
+    // ------------------------------------------------------------------------------------------ output
+    const int quarter = warp - OUT_WARP0, r = quarter * 32 + lane;
+    const uint32_t ocol = tmem + ((uint32_t)(quarter * 32) << 16) + O_COL;
+    const int nrows = row_count(p);
+    const uint32_t leader_o = map_to_rank(smem_u32(o_empty), 0);
+    int items = 0;
+    for (int i = 0;; ++i) {
+      const int ib = i & 1;
+      if (!wait(&info_full[ib], (uint32_t)(i >> 1))) break;
+      const ItemInfo it = info[ib];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&info_empty[ib]));
+      if (it.row0 < 0) break;
+      TileIter ti;
+      ti.init(p, it);
+      int start;
+      bool pre;
+      const bool tiles = ti.next(p, start, pre);
+      const int row = it.row0 + (int)rank * p.rows + r;
+      const bool live = r < p.rows && row < nrows;
+      const int tok = live ? row / p.group : 0, head = it.head * p.group + (live ? row - tok * p.group : 0);
+      uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride;
+      float* part = p.part_o + (((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * p.rows) + row) * D;
+      if (!wait(l_full, (uint32_t)i)) break;
+      const float inv = inv_l[r];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(l_empty));
+      if (tiles && !wait(o_full, (uint32_t)items)) break;
+      const f32x2 inv2 = x2_pack(inv, inv);
+      f32x2 check = 0ull;                        // becomes NaN with the first value that is not finite
+      if (__any_sync(0xffffffffu, live)) {
         tc_fence_after();
-        constexpr int HC = D / 2;
-        const int head = it.head * p.group + (row - tok * p.group);
-        const int64_t part_row = ((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * p.rows) + row;
-        const float inv = none ? 0.0f : 1.0f / l;
-        const f32x2 inv2 = x2_pack(inv, inv);
-        uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride + half * HC;
-        f32x2 check = 0ull;                      // becomes NaN with the first value that is not finite
 #pragma unroll 1
-        for (int x = 0; x < HC; x += 32) {
+        for (int x = 0; x < D; x += 32) {
           uint32_t o[32];
-          if (j > 0) {
-            tc_ld_32x32b_x32(ocol + half * HC + x, o);
+          if (tiles) {
+            tc_ld_32x32b_x32(ocol + x, o);
             tc_wait_ld(o);
           } else {
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = 0u;
           }
           if (p.parts > 1) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + part_row * D + half * HC + x);
             if (live) {
 #pragma unroll
               for (int y = 0; y < 8; ++y)
-                dst[y] = make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]), __uint_as_float(o[4 * y + 2]),
-                                     __uint_as_float(o[4 * y + 3]));
+                reinterpret_cast<float4*>(part + x)[y] =
+                    make_float4(__uint_as_float(o[4 * y]), __uint_as_float(o[4 * y + 1]), __uint_as_float(o[4 * y + 2]),
+                                __uint_as_float(o[4 * y + 3]));
             }
           } else {
             uint32_t v[2][8];
@@ -776,36 +816,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           __syncwarp();
         }
         tc_fence_before();
-        __syncwarp();
-        if (j > 0 && lane == 0) mbar_arrive_cluster(leader_o);
-        // 0 x (an infinity or NaN of a value that the row does not see) is NaN: such rows are done again key by key. A sum
-        // that is NaN itself came from a key that the row does see.
-        float x0, x1;
-        x2_unpack(check, x0, x1);
-        const uint32_t mine = __ballot_sync(0xffffffffu, live && l == l && !(x0 + x1 == 0.0f));
-        if (lane == 0) flags[half * 4 + quarter] = mine;
-        if (!(ok = meet())) break;
-        if (half == 0) {
-          if (p.parts > 1) {
-            if (live) p.part_ml[part_row] = make_float2(m, l);
-          } else {
-            if (live && p.a.lse != nullptr)
-              p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
-            uint32_t again = mine | flags[4 + quarter];
-#pragma unroll 1
-            while (again != 0u) {
-              const int src = __ffs(again) - 1;
-              again &= again - 1u;
-              row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src));
-            }
-          }
-        }
-      } else if (j > 0) {
-        if (!(ok = wait(o_full, (uint32_t)items))) break;
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_o);
       }
-      if (j > 0) ++items;
+      __syncwarp();
+      if (tiles) {
+        if (lane == 0) mbar_arrive_cluster(leader_o);
+        ++items;
+      }
+      // 0 x (an infinity or NaN of a value that the row does not see) is NaN: such rows are done again key by key. A sum that
+      // is NaN itself came from a key that the row does see.
+      float x0, x1;
+      x2_unpack(check, x0, x1);
+      uint32_t again = __ballot_sync(0xffffffffu, live && inv == inv && !(x0 + x1 == 0.0f));
+#pragma unroll 1
+      while (again != 0u) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1u;
+        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src));
+      }
     }
   }
   tc_fence_before();

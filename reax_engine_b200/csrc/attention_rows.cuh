@@ -18,7 +18,7 @@ struct RowKeys {
 };
 
 // the last b of [b0, b1) with cu_q[b] <= t (sequences of no rows are passed over); t < cu_q[b1]
-__device__ __noinline__ int sequence_of(const reaxmoe_attention_args& a, int t, int b0, int b1) {
+__device__ __forceinline__ int sequence_of(const reaxmoe_attention_args& a, int t, int b0, int b1) {
 #pragma unroll 1
   while (b1 - b0 > 1) {
     const int mid = (b0 + b1) >> 1;
@@ -44,7 +44,7 @@ __device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a,
 
 // Keys that query token t of sequence b sees. The cumulative lengths are cut to the tensors, so that no value of theirs makes
 // a later access leave them.
-__device__ __noinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
+__device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
   const int kt = (int)a.k_tokens, P = (int)a.prefix;
   const int ks = min(max(__ldg(a.cu_k + b), 0), kt);
   const int n = min(max(__ldg(a.cu_k + b + 1), ks), kt) - ks;
@@ -84,7 +84,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // reads the keys that the row sees and no others, which the tensor-core kernel cannot do where a tile of keys ends inside
 // what a row sees: there a masked key has weight 0, and 0 x (an infinity or NaN of its value) would be NaN.
 template <int D, bool BF>
-__device__ __noinline__ void row_by_warp(const reaxmoe_attention_args& a, int t, int head) {
+__device__ __forceinline__ void row_by_warp(const reaxmoe_attention_args& a, int t, int head) {
   constexpr int W = D / 64;                      // 32-bit words per lane
   const int lane = threadIdx.x & 31;
   const int kvh = head / (a.q_heads / a.kv_heads);
