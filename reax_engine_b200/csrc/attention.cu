@@ -67,8 +67,8 @@ struct ItemInfo {
   int head, part;    // KV head, part of the keys
   int p_lo, p_hi;    // prefix keys of this part
   int o_lo, o_hi;    // own keys of this part
-  int gap;           // keys that no row sees may lie between those of two sequences
-  __device__ __forceinline__ int tiles() const { return (p_hi - p_lo + KT - 1) / KT + (o_hi - o_lo + KT - 1) / KT; }   // no gap
+  int gap;           // keys that no row sees lie between those of two sequences
+  int tiles;         // of 128 keys each
 };
 
 struct Params {
@@ -89,57 +89,55 @@ __device__ __forceinline__ int row_count(const Params& p) {
   return max(t, 0) * p.group;
 }
 
-// The tiles of an item in order: prefix tiles, then own tiles, each 128 keys from `start`. Where own keys that no row sees may
-// lie between (gap), tiles begin at the first key that some row still needs; that is found by walking the tile's sequences.
+// The tiles of an item in order: prefix tiles, then own tiles, each 128 keys from `start`. Where own keys that no row sees lie
+// between two sequences' (gap), a tile begins at the first key that some row still needs, found by walking the sequences.
 struct TileIter {
-  int pc, ph, oc, oh;
-  int b, b_end, t0, t1, lo, hi;
-  bool gap;
-  __device__ __forceinline__ void need(const reaxmoe_attention_args& a) {
-    const int q0 = __ldg(a.cu_q + b), q1 = __ldg(a.cu_q + b + 1);
-    const int f = max(t0, q0), l = min(t1, q1) - 1;
-    lo = 0;
-    hi = 0;
-    if (f <= l) {
-      lo = row_keys_of(a, b, f).k_lo;
-      hi = row_keys_of(a, b, l).k_hi;
-    }
+  int cur, end, o_lo, o_hi;
+  int b, b1, t0, t1, lo, hi;
+  bool pre, gap;
+  __device__ __forceinline__ void need(const reaxmoe_attention_args& a) {    // own keys that the tile's rows of sequence b see
+    const int f = max(t0, __ldg(a.cu_q + b)), l = min(t1, __ldg(a.cu_q + b + 1)) - 1;
+    lo = row_keys_of(a, b, f).k_lo;
+    hi = row_keys_of(a, b, l).k_hi;
+    if (f > l || lo >= hi) lo = hi = 0;
+  }
+  __device__ __forceinline__ void own() {
+    pre = false;
+    cur = o_lo;
+    end = o_hi;
   }
   __device__ __forceinline__ void init(const Params& p, const ItemInfo& it) {
-    pc = it.p_lo;
-    ph = it.p_hi;
-    oc = it.o_lo;
-    oh = it.o_hi;
+    o_lo = it.o_lo;
+    o_hi = it.o_hi;
     gap = it.gap != 0;
     if (gap) {
       t0 = it.row0 / p.group;
       t1 = min(it.row0 + 2 * p.rows, row_count(p)) / p.group;
       b = it.b0;
-      b_end = it.b1;
+      b1 = it.b1;
       need(p.a);
     }
+    pre = true;
+    cur = it.p_lo;
+    end = it.p_hi;
+    if (cur >= end) own();
   }
-  __device__ __forceinline__ bool next(const Params& p, int& start, bool& pre) {
-    if (pc < ph) {
-      start = pc;
-      pre = true;
-      pc += KT;
-      return true;
-    }
-    pre = false;
-    if (gap) {
+  // one of the item's tiles: called it.tiles times at most
+  __device__ __forceinline__ int next(const Params& p) {
+    if (gap && !pre) {
 #pragma unroll 1
-      while (hi <= oc) {
-        if (b >= b_end) return false;
+      while (hi <= cur && b < b1) {
         ++b;
         need(p.a);
       }
-      oc = max(oc, lo);
+      cur = max(cur, lo);
     }
-    if (oc >= oh) return false;
-    start = oc;
-    oc += KT;
-    return true;
+    const int start = cur;
+    cur += KT;
+    return start;
+  }
+  __device__ __forceinline__ void after() {        // after each tile
+    if (pre && cur >= end) own();
   }
 };
 
@@ -157,9 +155,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   using L = Layout<D>;
   constexpr int NS = L::SLOTS, NB = L::NB, AHEAD = NB - 1;   // S tiles multiplied ahead of the softmax
   constexpr int O_COL = L::O_COL;
-  constexpr float THR = BF ? 8.0f : 3.0f;     // the maximum in use may lag behind by a factor of 2^THR before O is rescaled
-  // fp16 weights are shifted up by 2^12 (at most 2^15 with the lag), so that weights down to 2^-26 of the largest keep all bits
-  constexpr float SHIFT = BF ? 0.0f : 12.0f;
+  // The maximum in use may lag behind by a factor of 2^THR before O is rescaled, which costs a wait for the product before.
+  // Weights in bf16 keep their precision at any size, so only the range of the fp32 sums limits the lag. fp16 weights end at
+  // 2^16; they are shifted up by 2^SHIFT, so that weights down to 2^-18 of the one at the maximum in use keep all bits (a lag
+  // of 2^3 at SHIFT 12, which has 2^-26, made rescaling so frequent that D = 64 took 4500 clocks a tile).
+  constexpr float THR = BF ? 64.0f : 11.0f;
+  constexpr float SHIFT = BF ? 0.0f : 4.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
   uint64_t* full = bars;               // [NS] (leader's) both CTAs' halves landed (tx)
@@ -239,11 +240,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   if (warp == 8) {
     // ------------------------------------------------------------------------------------------ K / V producer
     if (elect_one()) {
-      int n = 0;                          // slots filled
+      int s = 0, n = 0;                   // ring position, slots filled
+      uint32_t sphase = 1;                // the first round finds the slots empty
       bool ok = true;
       auto fill = [&](bool value, int start, bool pre, int head) {
-        const int s = n % NS;
-        if (n >= NS && !wait1(&empty[s], (uint32_t)(n / NS - 1))) return false;
+        if (n >= NS && !wait1(&empty[s], sphase)) return false;
         const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
         const uint32_t dst = smem_u32(smem + L::ring + s * L::SLOT);
         if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * L::SLOT);
@@ -259,6 +260,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
             tma_load_3d_pair(dst + c * (KT * W * 2), tm, bar, (int)rank * (D / 2) + c * W, head, start);
         }
         ++n;
+        if (++s == NS) {
+          s = 0;
+          sphase ^= 1u;
+        }
         return true;
       };
       for (int i = 0; ok; ++i) {
@@ -268,20 +273,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         mbar_arrive(smem_u32(&info_empty[ib]));
         if (it.row0 < 0) break;
         // K tiles run AHEAD tiles before their V tiles
-        TileIter ki, vi;
-        ki.init(p, it);
-        vi.init(p, it);
-        int ks, vs, ahead = 0;
-        bool kp, vp, more = true;
-        while (ok) {
-          if (more) more = ki.next(p, ks, kp);
-          if (more) ok = fill(false, ks, kp, it.head);
-          if (ahead < AHEAD && more) {
-            ++ahead;
-            continue;
+        TileIter ti;
+        ti.init(p, it);
+        int start[AHEAD + 1];
+        bool pre[AHEAD + 1];
+#pragma unroll 1
+        for (int j = 0; ok && j < it.tiles + AHEAD; ++j) {
+#pragma unroll
+          for (int a = AHEAD; a > 0; --a) {
+            start[a] = start[a - 1];
+            pre[a] = pre[a - 1];
           }
-          if (!ok || !vi.next(p, vs, vp)) break;
-          ok = fill(true, vs, vp, it.head);
+          if (j < it.tiles) {
+            start[0] = ti.next(p);
+            pre[0] = ti.pre;
+            ti.after();
+            ok = fill(false, start[0], pre[0], it.head);
+          }
+          if (ok && j >= AHEAD) ok = fill(true, start[AHEAD], pre[AHEAD], it.head);
         }
       }
       // let the last loads land before the CTA may exit (only matters after an abort)
@@ -299,13 +308,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       const uint64_t vd = desc_v<D>(smem_u32(smem + L::ring));
       int slot = 0, items = 0;            // ring position, items with tiles
       uint32_t sphase = 0;
-      int gk = 0, gv = 0;                 // tiles multiplied with K, with V
+      int kbuf = 0, vbuf = 0, gv = 0;     // S buffers written and weighed with; tiles multiplied with V
+      uint32_t vphase = 0;
       bool ok = true;
       auto qk = [&]() {
         if (!wait1(&full[slot], sphase)) return false;
         tc_fence_after();
         const uint64_t b = kd + (uint64_t)(slot * (L::SLOT >> 4));
-        const uint32_t d = tmem + (uint32_t)(gk % NB * KT);
+        const uint32_t d = tmem + (uint32_t)(kbuf * KT);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -313,8 +323,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
             mma_pair_ss(d, qd + (uint64_t)((c * 16384 + k * 32) >> 4), b + (uint64_t)((c * 8192 + k * 32) >> 4), kQK,
                         (c | k) != 0 ? 1u : 0u);
         commit_pair(smem_u32(&empty[slot]));
-        commit_pair(smem_u32(&s_full[gk % NB]));
-        ++gk;
+        commit_pair(smem_u32(&s_full[kbuf]));
+        if (++kbuf == NB) kbuf = 0;
         if (++slot == NS) {
           slot = 0;
           sphase ^= 1u;
@@ -327,47 +337,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         const ItemInfo it = info[ib];
         mbar_arrive(smem_u32(&info_empty[ib]));
         if (it.row0 < 0) break;
-        TileIter ti;
-        int left = 0, start;
-        bool pre;
-        if (it.gap) ti.init(p, it); else left = it.tiles();
-        auto next = [&]() { return it.gap ? ti.next(p, start, pre) : left-- > 0; };
-        bool more = next();
-        if (!more) continue;
+        if (it.tiles == 0) continue;
         if (!(ok = wait1(q_full, (uint32_t)items))) break;
-        int ahead = 0;
-        for (; more && ahead < AHEAD; ++ahead) {
-          if (!(ok = qk())) break;
-          more = next();
-        }
-        if (!ok) break;
-        bool first = true, q_used = true;
-        while (ahead > 0) {
-          if (more) {
-            if (!(ok = qk())) break;
-            ++ahead;
-            more = next();
-          }
-          if (!more && q_used) {
-            commit_pair(smem_u32(q_empty));
-            q_used = false;
-          }
+#pragma unroll 1
+        for (int j = 0; j < it.tiles + AHEAD; ++j) {
+          if (j < it.tiles && !(ok = qk())) break;
+          if (j == it.tiles - 1) commit_pair(smem_u32(q_empty));
+          if (j < AHEAD) continue;
           if (!(ok = wait1(&full[slot], sphase))) break;
-          if (first && items > 0 && !(ok = wait1(o_empty, (uint32_t)(items - 1)))) break;
-          if (!(ok = wait1(&p_full[gv % NB], (uint32_t)(gv / NB)))) break;
+          if (j == AHEAD && items > 0 && !(ok = wait1(o_empty, (uint32_t)(items - 1)))) break;
+          if (!(ok = wait1(&p_full[vbuf], vphase))) break;
           tc_fence_after();
           const uint64_t b = vd + (uint64_t)(slot * (L::SLOT >> 4));
-          const uint32_t a = tmem + (uint32_t)(gv % NB * KT);
+          const uint32_t a = tmem + (uint32_t)(vbuf * KT);
 #pragma unroll
           for (int k = 0; k < KT / 16; ++k)
             mma_pair_ts(tmem + O_COL, a + k * 8, b + (uint64_t)((k * (D == 64 ? 1024 : 2048)) >> 4), kPV,
-                        first && k == 0 ? 0u : 1u);
+                        j == AHEAD && k == 0 ? 0u : 1u);
           commit_pair(smem_u32(&empty[slot]));
           commit_pair(smem_u32(&pv_done[gv & 1]));
-          if (ahead == 1) commit_pair(smem_u32(o_full));
-          first = false;
+          if (j == it.tiles + AHEAD - 1) commit_pair(smem_u32(o_full));
           ++gv;
-          --ahead;
+          if (++vbuf == NB) {
+            vbuf = 0;
+            vphase ^= 1u;
+          }
           if (++slot == NS) {
             slot = 0;
             sphase ^= 1u;
@@ -461,17 +455,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         it.o_lo = a1 > np ? klo + max(a0 - np, 0) * KT : 0;
         it.o_hi = a1 > np ? (a1 == np + no ? khi : klo + (a1 - np) * KT) : 0;
         it.gap = klo < khi && (unsigned)(khi - klo) - sum >= (unsigned)KT ? 1 : 0;
+        it.tiles = (it.p_hi - it.p_lo + KT - 1) / KT;
+        if (!it.gap) {
+          it.tiles += max(it.o_hi - it.o_lo + KT - 1, 0) / KT;
+        } else {
+          // as TileIter goes over them
+          TileIter ti;
+          ti.init(p, it);
+          int cur = it.o_lo;
+#pragma unroll 1
+          while (cur < it.o_hi) {
+            cur = max(cur, ti.lo);
+            const int hi = min(ti.hi, it.o_hi);
+            if (cur < hi) {
+              const int n = (hi - cur + KT - 1) / KT;
+              it.tiles += n;
+              cur += n * KT;
+            }
+            if (ti.b >= ti.b1) break;
+            ++ti.b;
+            ti.need(p.a);
+          }
+        }
       }
       if (lane == 0) {
         info[ib] = it;
         mbar_arrive(smem_u32(&info_full[ib]));
       }
       __syncwarp();
-      TileIter ti;
-      ti.init(p, it);
-      int start;
-      bool pre;
-      if (!ti.next(p, start, pre)) continue;
+      if (it.tiles == 0) continue;
       if (items > 0 && !wait(q_empty, (uint32_t)(items - 1))) break;
       if (lane == 0) {
         if (rank == 0) mbar_expect_tx(smem_u32(q_full), (uint32_t)(2 * D * 2 * p.rows));
@@ -497,7 +509,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     const uint32_t p_full0 = map_to_rank(smem_u32(&p_full[0]), 0);
     const uint32_t x_mine = smem_u32(smem + L::words) + (uint32_t)(half * ROWS + r) * 4;
     const uint32_t x_other = smem_u32(smem + L::words) + (uint32_t)((half ^ 1) * ROWS + r) * 4;
-    int g = 0, x_n = 0;
+    int g = 0, buf = 0, x_n = 0;          // tiles done, S buffer, exchanges
+    uint32_t sphase = 0;
     bool ok = true;
 
     ItemInfo it, it_next;
@@ -586,7 +599,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       float m = -INFINITY, l = 0.0f;             // the maximum in use (of scores times c), the sum of this half's weights
       TileIter ti;
       ti.init(p, it);
-      int j = 0;
       // what the warp's rows see of the prefix and of their own keys: all of them [f_lo, f_hi), none anything outside [s_lo, s_hi)
       struct Range { int f_lo, f_hi, s_lo, s_hi; };
       auto range = [&](int lo, int hi) {
@@ -603,9 +615,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         uint32_t seen0, seen1;                   // if not full: which of this thread's 64 columns its row sees
       } cur;
       auto next = [&](Tile& t) {
-        int start;
-        bool pre;
-        if (!ti.next(p, start, pre)) return false;
+        const int start = ti.next(p);
+        const bool pre = ti.pre;
+        ti.after();
         t.full = pre ? start >= pr.f_lo && start + KT <= pr.f_hi : start >= kr.f_lo && start + KT <= kr.f_hi;
         t.some = pre ? start < pr.s_hi && start + KT > pr.s_lo : start < kr.s_hi && start + KT > kr.s_lo;
         t.any0 = t.any1 = true;
@@ -621,15 +633,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           t.any0 = __any_sync(0xffffffffu, t.seen0 != 0u);
           t.any1 = __any_sync(0xffffffffu, t.seen1 != 0u);
         }
-        return true;
       };
       uint32_t s0[32], s1[32];
       float mine = -INFINITY;
-      auto scol = [&](int tile) { return tmem + lanes + (uint32_t)(tile % NB * KT); };
-      auto load = [&](int tile, uint32_t (&x0)[32], uint32_t (&x1)[32]) {   // of the tile's scores, this half's columns
+      auto scol = [&]() { return tmem + lanes + (uint32_t)(buf * KT); };
+      auto load = [&](uint32_t (&x0)[32], uint32_t (&x1)[32]) {            // of the tile's scores, this half's columns
         tc_fence_after();
-        tc_ld_32x32b_x32(scol(tile) + half * 64, x0);
-        tc_ld_32x32b_x32(scol(tile) + half * 64 + 32, x1);
+        tc_ld_32x32b_x32(scol() + half * 64, x0);
+        tc_ld_32x32b_x32(scol() + half * 64 + 32, x1);
       };
       auto find_max = [&](const Tile& t, uint32_t (&x0)[32], uint32_t (&x1)[32]) {
         tc_wait_ld(x0);
@@ -675,8 +686,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         const float mc = (m == -INFINITY ? 0.0f : m) - SHIFT;
         f32x2 sum[2] = {0ull, 0ull};
         // P takes the place of the first 64 columns of S, which both halves have read
-        weights(x0, t.any0, mc, sum, scol(g) + half * 32);
-        weights(x1, t.any1, mc, sum, scol(g) + half * 32 + 16);
+        weights(x0, t.any0, mc, sum, scol() + half * 32);
+        weights(x1, t.any1, mc, sum, scol() + half * 32 + 16);
         float y0, y1;
         x2_unpack(x2_add(sum[0], sum[1]), y0, y1);
         l += y0 + y1;
@@ -686,8 +697,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         uint32_t z[16];
 #pragma unroll
         for (int x = 0; x < 16; ++x) z[x] = 0u;
-        tc_st_32x32b_x16(scol(g) + half * 32, z);
-        tc_st_32x32b_x16(scol(g) + half * 32 + 16, z);
+        tc_st_32x32b_x16(scol() + half * 32, z);
+        tc_st_32x32b_x16(scol() + half * 32 + 16, z);
       };
       auto done = [&]() {
         if (any_live) {
@@ -695,17 +706,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(p_full0 + (uint32_t)(g % NB * 8));
+        if (lane == 0) mbar_arrive_cluster(p_full0 + (uint32_t)(buf * 8));
         ++g;
-        ++j;
+        if (++buf == NB) {
+          buf = 0;
+          sphase ^= 1u;
+        }
       };
-      bool more = next(cur);
+      if (it.tiles > 0) next(cur);
 #pragma unroll 1
-      while (more) {
-        if (!(ok = wait(&s_full[g % NB], (uint32_t)(g / NB)))) break;
+      for (int left = it.tiles; left > 0; --left) {
+        if (!(ok = wait(&s_full[buf], sphase))) break;
         if (any_live) {
           if (cur.some) {
-            load(g, s0, s1);
+            load(s0, s1);
             find_max(cur, s0, s1);
             if (!(ok = weigh(cur, s0, s1))) break;
           } else {
@@ -713,7 +727,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           }
         }
         done();
-        more = next(cur);
+        if (left > 1) next(cur);
       }
       if (!ok) break;
       // the sums, for the output warps
@@ -754,11 +768,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&info_empty[ib]));
       if (it.row0 < 0) break;
-      TileIter ti;
-      ti.init(p, it);
-      int start;
-      bool pre;
-      const bool tiles = ti.next(p, start, pre);
+      const bool tiles = it.tiles > 0;
       const int row = it.row0 + (int)rank * p.rows + r;
       const bool live = r < p.rows && row < nrows;
       const int tok = live ? row / p.group : 0, head = it.head * p.group + (live ? row - tok * p.group : 0);
@@ -847,7 +857,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
 // Joins the parts of a row: one warp per row.
 template <int D, bool BF>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
-  constexpr float SHIFT = BF ? 0.0f : 12.0f;
+  constexpr float SHIFT = BF ? 0.0f : 4.0f;      // as in pair_kernel
   constexpr int W = D / 32;
   const int id = (int)(blockIdx.x * 8 + (threadIdx.x >> 5));     // fits: the rows of fewer tiles than there are pairs
   const int lane = threadIdx.x & 31;

@@ -47,18 +47,15 @@ __device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a,
 __device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
   const int kt = (int)a.k_tokens, P = (int)a.prefix;
   const int ks = min(max(__ldg(a.cu_k + b), 0), kt);
-  const int n = min(max(__ldg(a.cu_k + b + 1), ks), kt) - ks;
-  const int64_t pos = (int64_t)P + n - ((int64_t)__ldg(a.cu_q + b + 1) - t);    // prefix + n - m + i
-  const int64_t all = (int64_t)P + n;
-  int64_t hi = a.causal ? pos + 1 : all;
-  int64_t lo = a.window > 0 ? pos - a.window + 1 : 0;
-  hi = hi < 0 ? 0 : (hi > all ? all : hi);
-  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
+  const int all = P + min(max(__ldg(a.cu_k + b + 1), ks), kt) - ks;
+  const int pos = all - (__ldg(a.cu_q + b + 1) - t);             // prefix + n - m + i
+  const int hi = a.causal ? min(max(pos, -1) + 1, all) : all;
+  const int lo = a.window > 0 && pos >= a.window ? min(pos - a.window + 1, hi) : 0;
   RowKeys r;
-  r.p_lo = (int)(lo < P ? lo : P);
-  r.p_hi = (int)(hi < P ? hi : P);
-  r.k_lo = ks + (int)(lo > P ? lo - P : 0);
-  r.k_hi = ks + (int)(hi > P ? hi - P : 0);
+  r.p_lo = min(lo, P);
+  r.p_hi = min(hi, P);
+  r.k_lo = ks + max(lo - P, 0);
+  r.k_hi = ks + max(hi - P, 0);
   return r;
 }
 __device__ __forceinline__ RowKeys row_keys(const reaxmoe_attention_args& a, int t) {
