@@ -202,8 +202,8 @@ typedef struct reaxmoe_attention_args {
   float scale;                /* > 0 */
 } reaxmoe_attention_args;
 
-/* Bytes of workspace reaxmoe_attention needs for these sizes (at least 256; 0 on bad sizes). It depends on the sizes alone,
- * not on the cumulative lengths. */
+/* Bytes of workspace reaxmoe_attention needs for these sizes (0 on bad sizes; 16: none is touched, any 16 bytes will do). It
+ * depends on the sizes and the SM budget alone, not on the cumulative lengths. One call at a time may use a workspace. */
 size_t reaxmoe_attention_workspace_size(const reaxmoe_attention_args* args);
 int reaxmoe_attention(const reaxmoe_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 

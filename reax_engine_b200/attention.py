@@ -16,21 +16,38 @@ import math
 import torch
 
 from . import _lib as L
-from .moe import _ptr, _require_cuda, _stream
+from .moe import _require_cuda
 
 _DTYPES = {torch.bfloat16: L.BF16, torch.float16: L.FP16}
 
+# What the checks of a call found for one set of shapes, strides, types and options: the argument block without its pointers
+# and the workspace's size. Emptied when the SM budget changes, on which the size depends.
+_checked: dict = {}
+_unused: dict = {}        # device -> the workspace of calls that use none
+_CHECKED_MAX = 4096
+_UNUSED = 16             # a workspace of this size is never touched (reaxmoe_attention_workspace_size)
+
+
+def forget_checked() -> None:
+    _checked.clear()
+
+
+def _readable(t: torch.Tensor) -> bool:
+    """t [tokens, heads, dim] as the kernels can address it: rows of contiguous elements that start on 16 bytes and do not
+    overlap (a view of a fused projection is)."""
+    n, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    return (s2 == 1 and t.data_ptr() % 16 == 0 and s0 % 8 == 0 and s1 % 8 == 0 and (h <= 1 or s1 >= d)
+            and (n <= 1 or s0 >= d))
+
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
-    """t [tokens, heads, dim] as the kernels can read it: rows of contiguous elements that start on 16 bytes and do not
-    overlap (a view of a fused projection is); anything else is copied."""
-    n, h, d = t.shape
-    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
-          and (h <= 1 or t.stride(1) >= d) and (n <= 1 or t.stride(0) >= d))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    return t if _readable(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _lengths(cu: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
+    if cu.dtype is torch.int32 and cu.ndim == 1 and cu.device == device and cu.is_contiguous() and cu.numel() > 0:
+        return cu
     if cu.ndim != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32 [sequences + 1]")
     if cu.device != device:
@@ -38,20 +55,16 @@ def _lengths(cu: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
     return cu.to(torch.int32).contiguous()
 
 
-def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out, workspace, status):
+def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window):
+    """The argument block of these tensors without its pointers, and the workspace's size."""
     ts = [("q", q), ("k", k), ("v", v)] + ([] if prefix_k is None else [("prefix_k", prefix_k), ("prefix_v", prefix_v)])
-    _require_cuda(*[t for _, t in ts], cu_seqlens, cu_seqlens_k, out, workspace, status)
     if q.dtype not in _DTYPES:
         raise ValueError(f"q must be bf16 or fp16, not {q.dtype}")
     for n, t in ts:
-        if t.ndim != 3:
-            raise ValueError(f"{n} must be [tokens, heads, head_dim]")
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{n} must have the dtype and device of q")
         if t.shape[2] != q.shape[2] or (n != "q" and t.shape[1] != k.shape[1]):
             raise ValueError(f"{n} {tuple(t.shape)} does not go with q {tuple(q.shape)} and k {tuple(k.shape)}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{n} requires grad: this attention has no backward")
     if k.shape[0] != v.shape[0] or (prefix_k is not None and prefix_k.shape[0] != prefix_v.shape[0]):
         raise ValueError("keys and values must have the same number of tokens")
     d = q.shape[2]
@@ -60,42 +73,90 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         raise ValueError("scale must be positive and finite")
     if window is not None and (not causal or int(window) < 1):
         raise ValueError("window must be at least 1, with causal=True")
-    cu_q = _lengths(cu_seqlens, "cu_seqlens", q.device)
-    cu_k = cu_q if cu_seqlens_k is None else _lengths(cu_seqlens_k, "cu_seqlens_k", q.device)
-    if cu_k.numel() != cu_q.numel():
+    if seqs_k != seqs:
         raise ValueError("cu_seqlens and cu_seqlens_k must have the same length")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-            raise ValueError("out must have the shape, dtype and device of q")
-        if any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for _, t in ts):
-            raise ValueError("out must not share its storage with an input")
-    if status is not None and (status.dtype != torch.int32 or status.device != q.device or status.numel() < 1):
-        raise ValueError("status must be an int32 tensor on the device of q")
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    q_, k_, v_ = _heads(q), _heads(k), _heads(v)
-    pk = None if prefix_k is None else _heads(prefix_k)
-    pv = None if prefix_v is None else _heads(prefix_v)
-    ok = out.stride(2) == 1 and out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0 and out.stride(1) % 8 == 0
-    dst = out if ok else out.clone(memory_format=torch.contiguous_format)
-    strides = [x for t in (q_, k_, v_, pk, pv, dst) for x in ((0, 0) if t is None else (t.stride(0), t.stride(1)))]
-    args = L.AttentionArgs(_ptr(q_), _ptr(k_), _ptr(v_), _ptr(pk), _ptr(pv), _ptr(cu_q), _ptr(cu_k), _ptr(dst), _ptr(lse),
-                           _ptr(status), *strides, q.shape[0], k.shape[0], 0 if pk is None else pk.shape[0],
-                           cu_q.numel() - 1, q.shape[1], k.shape[1], d, _DTYPES[q.dtype], int(bool(causal)),
+    strides = [x for t in (q, k, v, prefix_k, prefix_v, dst) for x in ((0, 0) if t is None else t.stride()[:2])]
+    args = L.AttentionArgs(*([None] * 10), *strides, q.shape[0], k.shape[0], 0 if prefix_k is None else prefix_k.shape[0],
+                           seqs - 1, q.shape[1], k.shape[1], d, _DTYPES[q.dtype], int(bool(causal)),
                            0 if window is None else min(int(window), 0x7FFFFFFF), scale)
-    with torch.cuda.device(q.device):
-        need = L.lib().reaxmoe_attention_workspace_size(ctypes.byref(args))
-        if need == 0:
-            raise L.ReaxMoEError(L.ERR_BAD_SHAPE, L.last_error())
-        if workspace is None:
+    need = L.lib().reaxmoe_attention_workspace_size(ctypes.byref(args))
+    if need == 0:
+        raise L.ReaxMoEError(L.ERR_BAD_SHAPE, L.last_error())
+    return bytes(args), need
+
+
+def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out, workspace, status):
+    inputs = (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v)
+    for t in inputs:
+        if not t.is_cuda:
+            _require_cuda(t)
+        if t.ndim != 3:
+            raise ValueError("q, k, v and the prefix must be [tokens, heads, head_dim]")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
+    device = q.device
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out,
+                              workspace, status)
+    cu_q = _lengths(cu_seqlens, "cu_seqlens", device)
+    cu_k = cu_q if cu_seqlens_k is None else _lengths(cu_seqlens_k, "cu_seqlens_k", device)
+    if out is None:
+        dst = torch.empty(q.shape, dtype=q.dtype, device=device)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+            raise ValueError("out must have the shape, dtype and device of q")
+        if any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in inputs):
+            raise ValueError("out must not share its storage with an input")
+        s0, s1, s2 = out.stride()
+        ok = s2 == 1 and out.data_ptr() % 16 == 0 and s0 % 8 == 0 and s1 % 8 == 0
+        dst = out if ok else out.clone(memory_format=torch.contiguous_format)
+    if status is not None and (status.dtype != torch.int32 or status.device != device or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor on the device of q")
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    if prefix_k is not None:
+        prefix_k, prefix_v = _heads(prefix_k), _heads(prefix_v)
+    key = (device, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, dst.stride(),
+           cu_q.shape, cu_k.shape, scale, causal, window, k.device, v.device)
+    if prefix_k is not None:
+        key += (prefix_k.shape, prefix_k.stride(), prefix_k.dtype, prefix_k.device, prefix_v.shape, prefix_v.stride(),
+                prefix_v.dtype, prefix_v.device)
+    found = _checked.get(key)
+    if found is None:
+        found = _check(q, k, v, prefix_k, prefix_v, cu_q.numel(), cu_k.numel(), dst, scale, causal, window)
+        if len(_checked) >= _CHECKED_MAX:
+            _checked.clear()
+        _checked[key] = found
+    block, need = found
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    if workspace is None:
+        if need <= _UNUSED:
+            workspace = _unused.get(device)
+            if workspace is None:
+                workspace = _unused[device] = torch.empty(_UNUSED, dtype=torch.uint8, device=device)
+        else:
             # of this call alone: ordered with the stream, and private to a graph that is being captured
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        elif workspace.device != q.device or not workspace.is_contiguous():
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        nbytes = need
+    else:
+        if workspace.device != device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous and on the device of q")
-        L.check(L.lib().reaxmoe_attention(ctypes.byref(args), workspace.data_ptr(),
-                                          workspace.numel() * workspace.element_size(), _stream(q.device)))
-    if dst is not out:
+        nbytes = workspace.numel() * workspace.element_size()
+    args = L.AttentionArgs.from_buffer_copy(block)
+    args.q, args.k, args.v, args.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), dst.data_ptr()
+    args.cu_q, args.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    if prefix_k is not None:
+        args.prefix_k, args.prefix_v = prefix_k.data_ptr(), prefix_v.data_ptr()
+    if lse is not None:
+        args.lse = lse.data_ptr()
+    if status is not None:
+        args.status = status.data_ptr()
+    rc = L.lib().reaxmoe_attention(ctypes.byref(args), workspace.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        L.check(rc)
+    if out is None:
+        out = dst
+    elif dst is not out:
         out.copy_(dst)
     return (out, lse) if return_lse else out
 

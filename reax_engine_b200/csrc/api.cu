@@ -1,5 +1,6 @@
 // api.cu -- the extern "C" entry points of include/reaxmoe.h: argument checks, workspace layout and the
 // launch sequence of the layer. No allocation, no host synchronisation on the forward path.
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -35,10 +36,15 @@ static int cuda_check(const char* what) {
 static int g_sm_budget = 0;   // 0: every SM (reaxmoe_set_sm_budget)
 
 static int num_sms() {
+  static std::atomic<int> known[64];        // per device; 0: not asked yet
   int dev = 0, n = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  if (n <= 0) n = 148;
+  if (dev >= 0 && dev < 64) n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (n <= 0) return (g_sm_budget > 0 && g_sm_budget < 148) ? g_sm_budget : 148;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  }
   return (g_sm_budget > 0 && g_sm_budget < n) ? g_sm_budget : n;
 }
 

@@ -29,6 +29,7 @@
 // Items (row tile, KV head, part of the keys) are taken in order, the first by pair number, further ones from a counter.
 // With few rows an item's keys are split over several pairs, which leave partial sums that combine_kernel joins.
 // All waits are bounded (globaltimer); a timeout records REAXMOE_ERR_DEVICE_TIMEOUT and the CTA winds down.
+#include <atomic>
 #include <cstring>
 
 #include "attention_rows.cuh"
@@ -64,6 +65,7 @@ struct Layout {
 struct ItemInfo {
   int row0;          // first row of the pair's tile; -1: no more items
   int b0, b1;        // first and last sequence that has rows in it
+  Sequence first;    // the first
   int head, part;    // KV head, part of the keys
   int p_lo, p_hi;    // prefix keys of this part
   int o_lo, o_hi;    // own keys of this part
@@ -97,8 +99,9 @@ struct TileIter {
   bool pre, gap;
   __device__ __forceinline__ void need(const reaxmoe_attention_args& a) {    // own keys that the tile's rows of sequence b see
     const int f = max(t0, __ldg(a.cu_q + b)), l = min(t1, __ldg(a.cu_q + b + 1)) - 1;
-    lo = row_keys_of(a, b, f).k_lo;
-    hi = row_keys_of(a, b, l).k_hi;
+    const Sequence s = sequence_at(a, b);
+    lo = row_keys_in(a, s, f).k_lo;
+    hi = row_keys_in(a, s, l).k_hi;
     if (f > l || lo >= hi) lo = hi = 0;
   }
   __device__ __forceinline__ void own() {
@@ -423,13 +426,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         // the union of the rows' ranges, sequence by sequence: from its first row's first key to its last row's last
         it.b0 = sequence_by_warp(p.a, t0);
         it.b1 = sequence_by_warp(p.a, t1 - 1);
+        it.first = sequence_at(p.a, it.b0);
         int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0;
         unsigned sum = 0;
 #pragma unroll 1
         for (int b = it.b0 + lane; b <= it.b1; b += 32) {
           const int f = max(t0, __ldg(p.a.cu_q + b)), l = min(t1, __ldg(p.a.cu_q + b + 1)) - 1;
           if (f > l) continue;
-          const RowKeys kf = row_keys_of(p.a, b, f), kl = row_keys_of(p.a, b, l);
+          const Sequence s = b == it.b0 ? it.first : sequence_at(p.a, b);
+          const RowKeys kf = row_keys_in(p.a, s, f), kl = row_keys_in(p.a, s, l);
           if (kf.p_lo < kl.p_hi) {
             plo = min(plo, kf.p_lo);
             phi = max(phi, kl.p_hi);
@@ -528,7 +533,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       tok_next = 0;
       if (it_next.row0 >= 0 && r < p.rows && row < nrows) {
         tok_next = row / p.group;
-        rk_next = row_keys_of(p.a, sequence_of(p.a, tok_next, it_next.b0, it_next.b1 + 1), tok_next);
+        rk_next = row_keys_in(p.a, it_next.b0 == it_next.b1 ? it_next.first
+                                       : sequence_at(p.a, sequence_of(p.a, tok_next, it_next.b0, it_next.b1 + 1)), tok_next);
       }
       return true;
     };
@@ -569,7 +575,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
 #pragma unroll
         for (int x = 0; x < 32; x += 2) {
           float e0, e1;
-          x2_unpack(x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm), e0, e1);
+          const f32x2 y = x2_fma(x2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), c2, nm);
+          x2_unpack(y, e0, e1);
           e0 = ex2(e0);
           e1 = ex2(e1);
           w[x / 2] = pack2<BF>(e0, e1);
@@ -597,32 +604,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       const bool any_live = __any_sync(0xffffffffu, live);
       const bool none = rk.p_lo >= rk.p_hi && rk.k_lo >= rk.k_hi;
       float m = -INFINITY, l = 0.0f;             // the maximum in use (of scores times c), the sum of this half's weights
-      TileIter ti;
-      ti.init(p, it);
-      // what the warp's rows see of the prefix and of their own keys: all of them [f_lo, f_hi), none anything outside [s_lo, s_hi)
-      struct Range { int f_lo, f_hi, s_lo, s_hi; };
-      auto range = [&](int lo, int hi) {
-        const bool e = lo >= hi;
-        return Range{__reduce_max_sync(0xffffffffu, lo), __reduce_min_sync(0xffffffffu, hi),
-                     __reduce_min_sync(0xffffffffu, e ? INT_MAX : lo), __reduce_max_sync(0xffffffffu, e ? 0 : hi)};
-      };
       // keys from the part's end on are the next part's, whose first tile may begin inside this one where there are gaps
       const int p_hi = min(rk.p_hi, it.p_hi), k_hi = min(rk.k_hi, it.o_hi);
-      const Range pr = range(rk.p_lo, p_hi), kr = range(rk.k_lo, k_hi);
+      // without gaps, tile j < np is the prefix's from p_lo + 128 j, the others are from o_lo + 128 (j - np); all rows of the
+      // warp see all of tiles [pf, pf + pn) and [kf, kf + kn)
+      const int np = (it.p_hi - it.p_lo + KT - 1) / KT;
+      int pf = 0, pn = 0, kf = 0, kn = 0;
+      TileIter ti;
+      if (it.gap) {
+        ti.init(p, it);
+      } else {
+        if (np > 0) {
+          pf = max(__reduce_max_sync(0xffffffffu, rk.p_lo) - it.p_lo + KT - 1, 0) / KT;
+          pn = max((__reduce_min_sync(0xffffffffu, p_hi) - it.p_lo) / KT - pf, 0);
+        }
+        if (it.tiles > np) {
+          kf = max(__reduce_max_sync(0xffffffffu, rk.k_lo) - it.o_lo + KT - 1, 0) / KT;
+          kn = max((__reduce_min_sync(0xffffffffu, k_hi) - it.o_lo) / KT - kf, 0);
+          kf += np;
+        }
+      }
       struct Tile {
         bool full, some;                         // all rows of the warp see all 128 keys; some row sees some key
         bool any0, any1;                         // some row sees some of this thread's first / last 32 columns
         uint32_t seen0, seen1;                   // if not full: which of this thread's 64 columns its row sees
       } cur;
-      auto next = [&](Tile& t) {
-        const int start = ti.next(p);
-        const bool pre = ti.pre;
-        ti.after();
-        t.full = pre ? start >= pr.f_lo && start + KT <= pr.f_hi : start >= kr.f_lo && start + KT <= kr.f_hi;
-        t.some = pre ? start < pr.s_hi && start + KT > pr.s_lo : start < kr.s_hi && start + KT > kr.s_lo;
-        t.any0 = t.any1 = true;
+      auto next = [&](Tile& t, int j) {
+        t.full = (unsigned)(j - pf) < (unsigned)pn || (unsigned)(j - kf) < (unsigned)kn;
+        t.some = t.any0 = t.any1 = true;
         if (!t.full) {
+          int start = j < np ? it.p_lo + j * KT : it.o_lo + (j - np) * KT;
+          bool pre = j < np;
+          if (it.gap) {
+            start = ti.next(p);
+            pre = ti.pre;
+            ti.after();
+          }
           const int a0 = (pre ? rk.p_lo : rk.k_lo) - start, a1 = (pre ? p_hi : k_hi) - start;   // columns [a0, a1) are seen
+          t.some = __any_sync(0xffffffffu, a0 < KT && a1 > max(a0, 0));
+          t.full = __all_sync(0xffffffffu, a0 <= 0 && a1 >= KT);
           auto seen = [&](int col) {                                   // of columns col .. col + 31
             const int f = min(max(a0 - col, 0), 32), e = min(max(a1 - col, 0), 32);
             const uint32_t below_e = e == 32 ? 0xffffffffu : (1u << e) - 1u, below_f = f == 32 ? 0xffffffffu : (1u << f) - 1u;
@@ -713,9 +733,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           sphase ^= 1u;
         }
       };
-      if (it.tiles > 0) next(cur);
+      if (it.tiles > 0) next(cur, 0);
 #pragma unroll 1
-      for (int left = it.tiles; left > 0; --left) {
+      for (int j = 0; j < it.tiles; ++j) {
         if (!(ok = wait(&s_full[buf], sphase))) break;
         if (any_live) {
           if (cur.some) {
@@ -727,7 +747,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           }
         }
         done();
-        if (left > 1) next(cur);
+        if (j + 1 < it.tiles) next(cur, j + 1);
       }
       if (!ok) break;
       // the sums, for the output warps
@@ -944,7 +964,7 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   pl.ml = 256;
   const size_t prow = pl.parts > 1 ? (size_t)pl.parts * a.kv_heads * pl.tiles * 2 * pl.rows : 0;
   pl.o = pl.ml + ((prow * 8 + 255) & ~size_t(255));
-  pl.total = pl.o + prow * a.head_dim * 4;
+  pl.total = pl.parts == 1 && pl.items <= pl.pairs ? 16 : pl.o + prow * a.head_dim * 4;
   return pl;
 }
 
@@ -977,8 +997,15 @@ static int launch_t(const AttentionLaunch& l, const Plan& pl, cudaStream_t s) {
        make_map_heads(&p.tmPV, a.prefix_v, a.prefix, a.prefix_v_stride, a.kv_heads, a.prefix_v_head_stride, D, VB, KT)))
     return REAXMOE_ERR_CUDA;
   auto kfn = pair_kernel<D, BF>;
-  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::total) != cudaSuccess)
-    return REAXMOE_ERR_CUDA;
+  static std::atomic<uint64_t> ready{0};        // devices on which the attribute is set (bit = device; others every time)
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return REAXMOE_ERR_CUDA;
+  const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+  if ((ready.load(std::memory_order_acquire) & bit) == 0) {
+    if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::total) != cudaSuccess)
+      return REAXMOE_ERR_CUDA;
+    ready.fetch_or(bit, std::memory_order_release);
+  }
   if (p.counter != nullptr && cudaMemsetAsync(p.counter, 0, sizeof(int), s) != cudaSuccess) return REAXMOE_ERR_CUDA;
   kfn<<<2 * pl.pairs, THREADS, Layout<D>::total, s>>>(p);
   if (pl.parts > 1) combine_kernel<D, BF><<<(unsigned)ceil_div64(a.q_tokens * a.q_heads, 8), 256, 0, s>>>(p);

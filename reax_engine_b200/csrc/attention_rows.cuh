@@ -42,21 +42,35 @@ __device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a,
   return b0;
 }
 
-// Keys that query token t of sequence b sees. The cumulative lengths are cut to the tensors, so that no value of theirs makes
-// a later access leave them.
-__device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
-  const int kt = (int)a.k_tokens, P = (int)a.prefix;
-  const int ks = min(max(__ldg(a.cu_k + b), 0), kt);
-  const int all = P + min(max(__ldg(a.cu_k + b + 1), ks), kt) - ks;
-  const int pos = all - (__ldg(a.cu_q + b + 1) - t);             // prefix + n - m + i
-  const int hi = a.causal ? min(max(pos, -1) + 1, all) : all;
+// A sequence: its first own key, prefix and own keys together, and the token behind its last query row. The cumulative lengths
+// are cut to the tensors, so that no value of theirs makes a later access leave them.
+struct Sequence {
+  int ks, all, q_end;
+};
+__device__ __forceinline__ Sequence sequence_at(const reaxmoe_attention_args& a, int b) {
+  const int kt = (int)a.k_tokens;
+  Sequence s;
+  s.ks = min(max(__ldg(a.cu_k + b), 0), kt);
+  s.all = (int)a.prefix + min(max(__ldg(a.cu_k + b + 1), s.ks), kt) - s.ks;
+  s.q_end = __ldg(a.cu_q + b + 1);
+  return s;
+}
+
+// Keys that its query token t sees.
+__device__ __forceinline__ RowKeys row_keys_in(const reaxmoe_attention_args& a, const Sequence& s, int t) {
+  const int P = (int)a.prefix;
+  const int pos = s.all - (s.q_end - t);                         // prefix + n - m + i
+  const int hi = a.causal ? min(max(pos, -1) + 1, s.all) : s.all;
   const int lo = a.window > 0 && pos >= a.window ? min(pos - a.window + 1, hi) : 0;
   RowKeys r;
   r.p_lo = min(lo, P);
   r.p_hi = min(hi, P);
-  r.k_lo = ks + max(lo - P, 0);
-  r.k_hi = ks + max(hi - P, 0);
+  r.k_lo = s.ks + max(lo - P, 0);
+  r.k_hi = s.ks + max(hi - P, 0);
   return r;
+}
+__device__ __forceinline__ RowKeys row_keys_of(const reaxmoe_attention_args& a, int b, int t) {
+  return row_keys_in(a, sequence_at(a, b), t);
 }
 __device__ __forceinline__ RowKeys row_keys(const reaxmoe_attention_args& a, int t) {
   return row_keys_of(a, sequence_of(a, t, 0, a.seqs), t);

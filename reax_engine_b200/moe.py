@@ -64,6 +64,8 @@ def set_sm_budget(sms: int) -> None:
     """Cap the library's persistent kernels at ``sms`` CTAs (0: every SM), leaving the rest of the device to work
     that runs beside them, such as overlapped NCCL exchanges. Process-wide."""
     L.lib().reaxmoe_set_sm_budget(int(sms))
+    from .attention import forget_checked      # workspace sizes depend on it
+    forget_checked()
 
 
 def route(hidden_states: torch.Tensor | None, gating_output: torch.Tensor, topk: int, renormalize: bool = True,

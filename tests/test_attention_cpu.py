@@ -22,7 +22,7 @@ def call(**kw):
 def test_a_good_call_needs_its_workspace():
     assert call() == L.ERR_WORKSPACE
     a = L.AttentionArgs(**BASE)
-    assert L.lib().reaxmoe_attention_workspace_size(ctypes.byref(a)) >= 256
+    assert L.lib().reaxmoe_attention_workspace_size(ctypes.byref(a)) >= 16
     assert L.lib().reaxmoe_attention(None, None, 0, None) == L.ERR_NULL
     assert L.lib().reaxmoe_attention_workspace_size(None) == 0
 

@@ -307,7 +307,7 @@ def test_workspace_and_status():
     a = R.prompt_attention(q, k, v, dev([0, 1]), dev([0, 4000]), workspace=ws, status=status)
     assert torch.equal(a, R.prompt_attention(q, k, v, dev([0, 1]), dev([0, 4000]))) and int(status) == 0
     with pytest.raises(L.ReaxMoEError) as e:
-        R.prompt_attention(q, k, v, dev([0, 1]), dev([0, 4000]), workspace=ws[:16])
+        R.prompt_attention(q, k, v, dev([0, 1]), dev([0, 4000]), workspace=ws[:64])
     assert e.value.code == L.ERR_WORKSPACE
 
 
