@@ -32,6 +32,7 @@
 #include <atomic>
 #include <cstring>
 
+#include "attention_few.cuh"
 #include "attention_rows.cuh"
 #include "attention_sm100.cuh"
 #include "kernels.cuh"
@@ -79,6 +80,8 @@ struct Params {
   int group;
   int rows;          // rows of a CTA's tile: group times the tokens that fit into 128
   int tiles, parts, items;
+  int prefix_only;   // own keys are left to few_kernel
+  int partial;       // partial sums are left for a joining kernel
   int wide_out;      // output rows start on 32 bytes
   int* counter;      // items taken beyond the first of each pair (null when there are none)
   float* part_o;     // [parts][kv_heads][tiles * 2 * rows][D]
@@ -439,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
             plo = min(plo, kf.p_lo);
             phi = max(phi, kl.p_hi);
           }
-          if (kf.k_lo < kl.k_hi) {
+          if (kf.k_lo < kl.k_hi && !p.prefix_only) {
             klo = min(klo, kf.k_lo);
             khi = max(khi, kl.k_hi);
             sum += (unsigned)(kl.k_hi - kf.k_lo);
@@ -764,7 +767,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         if (lane == 0) mbar_arrive(smem_u32(l_full));
         if (live) {
           const int in_group = row - tok * p.group;
-          if (p.parts > 1)
+          if (p.partial)
             p.part_ml[((int64_t)it.part * p.a.kv_heads + it.head) * ((int64_t)p.tiles * 2 * p.rows) + row] = make_float2(m, l);
           else if (p.a.lse != nullptr)
             p.a.lse[(int64_t)tok * p.a.q_heads + it.head * p.group + in_group] =
@@ -813,7 +816,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = 0u;
           }
-          if (p.parts > 1) {
+          if (p.partial) {
             if (live) {
 #pragma unroll
               for (int y = 0; y < 8; ++y)
@@ -938,10 +941,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
     p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
 }
 
-// Row tiles, parts of the keys, and the workspace: counter, partial maxima and sums, partial outputs.
+// Row tiles, parts of the keys, and the workspace: counter, partial maxima and sums, partial outputs (of pair_kernel, of
+// few_kernel).
 struct Plan {
   int group, rows, tiles, parts, items, pairs;
-  size_t ml, o, total;
+  bool few;
+  int chunk, units;
+  size_t ml, o, few_ml, few_o, total;
 };
 
 static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
@@ -952,7 +958,14 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   pl.tiles = (int)ceil_div64(rows, 2 * pl.rows);
   const int64_t base = (int64_t)pl.tiles * a.kv_heads;
   const int pairs = num_sms / 2 > 0 ? num_sms / 2 : 1;
-  const int64_t keys = a.prefix + a.k_tokens;
+  // A generation step (no more query tokens than sequences, with some keys each) goes to few_kernel: 64 sequences of about 1000
+  // keys take 62 us there against 211 in tiles at D = 64 (16 KV heads), 66 against 103 at D = 128 (8), 120 against 115 at
+  // D = 256 (8; 64 x 100 keys 24 against 28, one of 16000 36 against 40). With a prefix it is a launch more, which pays from
+  // some own keys on: 256 sequences of 64 behind 8000 60 against 81 us (D = 64), 85 against 80 (D = 128; of 300 behind 2000
+  // 101 against 134), at D = 256 not (64 of 500 behind 4000 94 against 73).
+  pl.few = pl.group <= FEW_ROWS && a.q_tokens <= a.seqs && a.k_tokens >= 16 * (int64_t)a.seqs && a.k_tokens > 0 &&
+           (a.prefix == 0 || (a.head_dim == 64 && a.k_tokens >= 4096) || (a.head_dim == 128 && a.k_tokens >= 32768));
+  const int64_t keys = a.prefix + (pl.few ? 0 : a.k_tokens);
   // split the keys when the tiles leave half of the pairs idle, into parts of at least 512 keys
   int64_t parts = base > 0 && base * 2 <= pairs ? pairs / base : 1;
   const int64_t most = ceil_div64(keys, 512);
@@ -961,11 +974,67 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   const int64_t items = base * pl.parts;
   pl.items = (int)items;
   pl.pairs = (int)(items < pairs ? items : pairs);
+  // units of few_kernel, of at least 64 keys: with few sequences one for every warp of the device (each sequence may have one
+  // more than its share), else about three, so that the ends of sequences even out
+  const int64_t warps = ceil_div64((int64_t)num_sms * FEW_WARPS, a.kv_heads);       // for each KV head
+  int64_t chunk = ceil_div64(a.k_tokens, warps >= 8 * (int64_t)a.seqs ? warps - a.seqs : 3 * warps);
+  chunk = chunk < 64 ? 64 : ceil_div64(chunk, 16) * 16;
+  pl.chunk = (int)chunk;
+  pl.units = pl.few ? (int)(ceil_div64(a.k_tokens, chunk) + a.seqs) : 0;
+  auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  const size_t prow = pl.parts > 1 || (pl.few && a.prefix > 0) ? (size_t)pl.parts * a.kv_heads * pl.tiles * 2 * pl.rows : 0;
+  const size_t frow = (size_t)pl.units * a.kv_heads * FEW_ROWS;
   pl.ml = 256;
-  const size_t prow = pl.parts > 1 ? (size_t)pl.parts * a.kv_heads * pl.tiles * 2 * pl.rows : 0;
-  pl.o = pl.ml + ((prow * 8 + 255) & ~size_t(255));
-  pl.total = pl.parts == 1 && pl.items <= pl.pairs ? 16 : pl.o + prow * a.head_dim * 4;
+  pl.o = up(pl.ml + prow * 8);
+  pl.few_ml = up(pl.o + prow * a.head_dim * 4);
+  pl.few_o = up(pl.few_ml + frow * 8);
+  pl.total = prow == 0 && frow == 0 && pl.items <= pl.pairs ? 16 : pl.few_o + frow * a.head_dim * 4;
   return pl;
+}
+
+// the kernel's dynamic shared memory, allowed once per device (bit = device; devices from 64 on every time)
+template <typename K>
+static int allow_smem(K kfn, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return REAXMOE_ERR_CUDA;
+  const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+  if ((done.load(std::memory_order_acquire) & bit) != 0) return 0;
+  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return REAXMOE_ERR_CUDA;
+  done.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
+template <int D, bool BF>
+static int launch_few(const AttentionLaunch& l, const Plan& pl, const Params* prefix, cudaStream_t s) {
+  const reaxmoe_attention_args& a = l.a;
+  uint8_t* ws = static_cast<uint8_t*>(l.workspace);
+  FewParams f;
+  memset(&f, 0, sizeof(f));
+  f.a = a;
+  f.group = pl.group;
+  f.chunk = pl.chunk;
+  f.units = pl.units;
+  f.ml = reinterpret_cast<float2*>(ws + pl.few_ml);
+  f.o = reinterpret_cast<float*>(ws + pl.few_o);
+  if (prefix != nullptr) {
+    f.prefix_parts = pl.parts;
+    f.prefix_rows = pl.tiles * 2 * pl.rows;
+    f.prefix_ml = prefix->part_ml;
+    f.prefix_o = prefix->part_o;
+  }
+  static std::atomic<uint64_t> allowed{0};
+  if (allow_smem(few_kernel<D, BF>, FewLayout<D>::total, allowed)) return REAXMOE_ERR_CUDA;
+  const int64_t tasks = (int64_t)pl.units * a.kv_heads;
+  const int64_t blocks = (int64_t)l.num_sms * FewLayout<D>::BLOCKS;
+  const int grid = (int)(tasks < blocks ? tasks : blocks);
+  few_kernel<D, BF><<<grid, FEW_WARPS * 32, FewLayout<D>::total, s>>>(f);
+  // partial results a row on the average: a warp joins up to about 32
+  const int64_t rows = a.q_tokens * a.q_heads, results = pl.units / a.seqs + (prefix != nullptr ? pl.parts : 0);
+  if (results <= 32)
+    join_kernel<D, BF, 1><<<(unsigned)ceil_div64(rows, JOIN_WARPS), JOIN_WARPS * 32, 0, s>>>(f);
+  else
+    join_kernel<D, BF, JOIN_WARPS><<<(unsigned)rows, JOIN_WARPS * 32, 0, s>>>(f);
+  return cudaPeekAtLastError() == cudaSuccess ? 0 : REAXMOE_ERR_CUDA;
 }
 
 template <int D, bool BF>
@@ -985,10 +1054,13 @@ static int launch_t(const AttentionLaunch& l, const Plan& pl, cudaStream_t s) {
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
   p.part_o = reinterpret_cast<float*>(ws + pl.o);
   p.timeout_ns = l.timeout_ns;
+  p.prefix_only = pl.few ? 1 : 0;
+  p.partial = pl.parts > 1 || pl.few ? 1 : 0;
+  if (pl.few && a.prefix == 0) return launch_few<D, BF>(l, pl, nullptr, s);
   constexpr int VB = D == 64 ? 32 : 64;
   if (make_map_rows(&p.tmQ, a.q, a.q_tokens, a.q_stride, a.kv_heads, pl.group, a.q_head_stride, D, pl.rows / pl.group))
     return REAXMOE_ERR_CUDA;
-  if (a.k_tokens > 0 &&
+  if (a.k_tokens > 0 && !pl.few &&
       (make_map_heads(&p.tmK, a.k, a.k_tokens, a.k_stride, a.kv_heads, a.k_head_stride, D, 64, 64) ||
        make_map_heads(&p.tmV, a.v, a.k_tokens, a.v_stride, a.kv_heads, a.v_head_stride, D, VB, KT)))
     return REAXMOE_ERR_CUDA;
@@ -996,18 +1068,11 @@ static int launch_t(const AttentionLaunch& l, const Plan& pl, cudaStream_t s) {
       (make_map_heads(&p.tmPK, a.prefix_k, a.prefix, a.prefix_k_stride, a.kv_heads, a.prefix_k_head_stride, D, 64, 64) ||
        make_map_heads(&p.tmPV, a.prefix_v, a.prefix, a.prefix_v_stride, a.kv_heads, a.prefix_v_head_stride, D, VB, KT)))
     return REAXMOE_ERR_CUDA;
-  auto kfn = pair_kernel<D, BF>;
-  static std::atomic<uint64_t> ready{0};        // devices on which the attribute is set (bit = device; others every time)
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return REAXMOE_ERR_CUDA;
-  const uint64_t bit = device < 64 ? 1ull << device : 0ull;
-  if ((ready.load(std::memory_order_acquire) & bit) == 0) {
-    if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::total) != cudaSuccess)
-      return REAXMOE_ERR_CUDA;
-    ready.fetch_or(bit, std::memory_order_release);
-  }
+  static std::atomic<uint64_t> allowed{0};
+  if (allow_smem(pair_kernel<D, BF>, Layout<D>::total, allowed)) return REAXMOE_ERR_CUDA;
   if (p.counter != nullptr && cudaMemsetAsync(p.counter, 0, sizeof(int), s) != cudaSuccess) return REAXMOE_ERR_CUDA;
-  kfn<<<2 * pl.pairs, THREADS, Layout<D>::total, s>>>(p);
+  pair_kernel<D, BF><<<2 * pl.pairs, THREADS, Layout<D>::total, s>>>(p);
+  if (pl.few) return launch_few<D, BF>(l, pl, &p, s);
   if (pl.parts > 1) combine_kernel<D, BF><<<(unsigned)ceil_div64(a.q_tokens * a.q_heads, 8), 256, 0, s>>>(p);
   return cudaPeekAtLastError() == cudaSuccess ? 0 : REAXMOE_ERR_CUDA;
 }

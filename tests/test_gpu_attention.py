@@ -161,6 +161,39 @@ def test_more_tiles_than_pairs():
             check(o[:, h:h + 1], reference(*one, c, c, d ** -0.5), lse[:, h:h + 1])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("q_lens,k_lens,hq,hk", [
+    ((1,) * 7, (40, 1, 700, 0, 16, 17, 300), 4, 2),
+    ((2, 0, 1, 0, 3), (100, 30, 64, 1, 200), 4, 1),          # several rows of a sequence, others without any
+    ((1, 1, 1), (130, 257, 90), 16, 1),                      # 16 rows a sequence
+    ((1, 1), (50, 60), 10, 2),
+    ((20,) + (0,) * 23, (500,) + (3,) * 23, 4, 2),           # more rows of a sequence than the generation step's kernel takes
+    ((1,) * 40, (64,) * 40, 2, 2),
+])
+@pytest.mark.parametrize("window,prefix", [(None, 0), (33, 0), (None, 150), (90, 40)])
+def test_generation_steps(q_lens, k_lens, hq, hk, window, prefix, d):
+    run(q_lens, k_lens, hq=hq, hk=hk, d=d, window=window, prefix=prefix, dtype="bf16" if d != 128 else "fp16", seed=len(q_lens) + d)
+
+
+def test_generation_step_beside_values_that_it_does_not_see():
+    import reax_engine_b200 as R
+    for d, hq, hk in ((64, 4, 2), (256, 2, 1)):
+        cq, ck = [0, 1, 2, 4], [0, 200, 203, 400]
+        q, k, v, pk, pv = tensors(6, 450, hq, hk, d, "bf16", d, prefix=70)
+        ref = reference(q, k, v, cq, ck, d ** -0.5, window=60, prefix_k=pk, prefix_v=pv)
+        k, v = k.clone(), v.clone()
+        for t in (k, v):
+            t[200:203] = float("nan")      # the whole second sequence
+            t[:130] = float("inf")         # before the window
+            t[399] = float("-inf")         # after the last row but one
+            t[400:] = float("nan")         # behind the last sequence
+        out = torch.full_like(q, 2.0)
+        _, lse = R.shared_prefix_attention(q, k, v, pk, pv, dev(cq), dev(ck), window=60, out=out, return_lse=True)
+        keep = torch.tensor([True, False, True, False])
+        check(out[:4].cpu()[keep], [r[:4][keep] for r in ref], lse[:4].cpu()[keep])
+        assert (out[4:] == 2).all() and torch.isnan(out[1].float()).any()
+
+
 def test_large_and_small_scores():
     """Scores of hundreds, whose running maximum grows from tile to tile, and weights far below the largest."""
     import reax_engine_b200 as R
@@ -171,6 +204,8 @@ def test_large_and_small_scores():
         for kk in (k, k.flip(0)):
             o, lse = R.prompt_attention(q, kk, v, dev(c), scale=0.7, return_lse=True)
             check(o, reference(q, kk, v, c, c, 0.7), lse)
+            o, lse = R.prompt_attention(q[:1], kk, v, dev([0, 1]), dev(c), scale=0.7, return_lse=True)
+            check(o, reference(q[:1], kk, v, [0, 1], c, 0.7), lse)
         flat = torch.zeros_like(q)      # every weight the same
         o, lse = R.prompt_attention(flat, k, v, dev(c), return_lse=True)
         check(o, reference(flat, k, v, c, c, 128 ** -0.5), lse)
