@@ -20,7 +20,10 @@ What runs where:
 * experts: :func:`reax_engine_b200.run_moe_nvfp4` (permute + NVFP4 grouped GEMMs + combine), on a second stream
   in parallel with the dense MLP of the same layer;
 * dense projections: bf16 cuBLAS GEMMs through torch; attention: flash-attention varlen (both library kernels, outside
-  the MoE path this library owns);
+  the MoE path this library owns), or with ``attention="native"`` :func:`reax_engine_b200.prompt_attention`;
+* prompts that continue one shared prefix (an instruction, a context): :meth:`DecisionModel.prefill_prefix` runs it once and
+  keeps its keys and values, :meth:`DecisionModel.forward` with ``prefix`` then runs only what follows it
+  (:func:`reax_engine_b200.shared_prefix_attention`);
 * the last layer computes its feed-forward blocks and its attention queries for the prompts' last rows only.
 
 Layer pattern: BASELINE config 3 says "alternating" sliding / global, so even layers slide and odd layers are global
@@ -34,6 +37,7 @@ import torch
 
 from . import _lib as L
 from . import moe as M
+from .attention import prompt_attention, shared_prefix_attention
 
 
 @dataclass
@@ -139,14 +143,28 @@ def gelu_tanh_mul(gu: torch.Tensor) -> torch.Tensor:
     return h
 
 
+@dataclass
+class PrefixState:
+    """A prefix that prompts continue: its keys and values of every layer, [length, kv_heads, head_dim] bf16 (after the norms
+    and RoPE at positions 0 .. length - 1)."""
+    length: int
+    keys: list
+    values: list
+
+
 class DecisionModel:
     """Random-init Gemma-4 26B-A4B-shaped model on one GPU (``device``). Weights are seeded and drawn on the
     device: linear weights and embeddings ~ N(0, init_std), norm weights 1, expert weights NVFP4-quantised from
-    N(0, init_std)."""
+    N(0, init_std). ``attention``: "library" (flash-attention varlen) or "native" (this library's attention; close to the other
+    within the rounding of bf16, not bit-identical)."""
 
-    def __init__(self, cfg: DecisionConfig, device, seed: int = 0):
-        from flash_attn import flash_attn_varlen_func
-        self._fa = flash_attn_varlen_func
+    def __init__(self, cfg: DecisionConfig, device, seed: int = 0, attention: str = "library"):
+        if attention not in ("library", "native"):
+            raise ValueError(f"attention must be 'library' or 'native', not {attention!r}")
+        self.attention = attention
+        if attention == "library":
+            from flash_attn import flash_attn_varlen_func
+            self._fa = flash_attn_varlen_func
         self.cfg = c = cfg
         self.dev = torch.device(device)
         if self.dev.type != "cuda":
@@ -232,12 +250,26 @@ class DecisionModel:
         self.max_positions = max_len
 
     def _attention(self, lw: LayerWeights, layer: int, xn: torch.Tensor, pos: torch.Tensor, cu: torch.Tensor,
-                   max_len: int, last: torch.Tensor | None) -> torch.Tensor:
+                   max_len: int, last: torch.Tensor | None, prefix: PrefixState | None = None,
+                   keep: PrefixState | None = None) -> torch.Tensor:
         c = self.cfg
         qkv = xn @ lw.wqkv.t()
         kind = "local" if c.sliding(layer) else "global"
         cos, sin = self._rope_cache[kind]
         q, k, v = qkv_norm_rope(qkv, lw.q_norm, lw.k_norm, cos, sin, pos, c.eps, c.heads, c.kv_heads, c.head_dim)
+        if keep is not None:
+            keep.keys.append(k)
+            keep.values.append(v)
+        if prefix is not None or keep is not None or self.attention == "native":
+            # the last query row of each prompt alone where `last` says so: the mask is aligned to the end of the keys
+            cu_q = cu if last is None else torch.arange(last.numel() + 1, dtype=torch.int32, device=self.dev)
+            kw = dict(scale=1.0, window=c.window if c.sliding(layer) else None)
+            qq = q if last is None else q[last]
+            if prefix is None:
+                o = prompt_attention(qq, k, v, cu_q, cu, **kw)
+            else:
+                o = shared_prefix_attention(qq, k, v, prefix.keys[layer], prefix.values[layer], cu_q, cu, **kw)
+            return o.reshape(o.shape[0], c.heads * c.head_dim) @ lw.wo.t()
         win = (c.window - 1, 0) if c.sliding(layer) else (-1, -1)
         if last is None:
             o = self._fa(q, k, v, cu, cu, max_len, max_len, softmax_scale=1.0, causal=True, window_size=win)
@@ -275,26 +307,15 @@ class DecisionModel:
     layer_log = None        # a list: per layer a dict of its input x, residual r, dense and MoE outputs; then the
                             # final rows
 
-    @torch.no_grad()
-    def forward(self, token_ids: torch.Tensor, cu_seqlens: torch.Tensor, option_ids: torch.Tensor,
-                temperature: float = 1.0) -> torch.Tensor:
-        """token_ids [N] (packed prompts), cu_seqlens [B + 1] int32 (device), option_ids [n_opt]. Returns the
-        option probabilities [B, n_opt] float64 at each prompt's last position."""
+    def _layers(self, x: torch.Tensor, pos: torch.Tensor, cu: torch.Tensor, max_len: int, last: torch.Tensor | None,
+                prefix: PrefixState | None = None, keep: PrefixState | None = None) -> torch.Tensor:
+        """All layers on x [n, hidden]; the last one for rows `last` only."""
         c = self.cfg
-        cu = cu_seqlens.to(device=self.dev, dtype=torch.int32)
-        n = token_ids.numel()
-        lens = cu[1:] - cu[:-1]
-        max_len = int(lens.max())
-        self._cos_sin(max_len)
-        seq = torch.repeat_interleave(torch.arange(lens.numel(), device=self.dev), lens.long(), output_size=n)
-        pos = torch.arange(n, device=self.dev) - cu[:-1].long()[seq]
-        last = (cu[1:] - 1).long()
-        x = self.embed[token_ids.to(self.dev).long()] * self.normalizer
         cur = torch.cuda.current_stream(self.dev)
         for i, lw in enumerate(self.layers):
             is_last = i == c.layers - 1
             rows = last if is_last else None
-            a = self._attention(lw, i, rms_norm(x, lw.norms["input"], c.eps), pos, cu, max_len, rows)
+            a = self._attention(lw, i, rms_norm(x, lw.norms["input"], c.eps), pos, cu, max_len, rows, prefix, keep)
             r = rms_norm(a, lw.norms["post_attention"], c.eps, residual=x[last] if is_last else x)
             # the MoE block on its own stream, in parallel with the dense MLP
             self.moe_stream.wait_stream(cur)
@@ -308,6 +329,43 @@ class DecisionModel:
             x = rms_norm(d, lw.norms["post_ff"], c.eps, b=m, residual=r)
             if lw.layer_scalar != 1.0:
                 x = x * lw.layer_scalar
+        return x
+
+    @torch.no_grad()
+    def prefill_prefix(self, token_ids: torch.Tensor) -> PrefixState:
+        """Runs a prefix [length] that prompts will continue and keeps every layer's keys and values for
+        :meth:`forward` (``prefix``). Its own attention is this library's, whatever ``attention`` says."""
+        n = token_ids.numel()
+        if n < 1:
+            raise ValueError("a prefix has at least one token")
+        self._cos_sin(n)
+        x = self.embed[token_ids.to(self.dev).long()] * self.normalizer
+        pos = torch.arange(n, device=self.dev)
+        cu = torch.tensor([0, n], dtype=torch.int32, device=self.dev)
+        state = PrefixState(n, [], [])
+        self._layers(x, pos, cu, n, torch.tensor([n - 1], device=self.dev), keep=state)
+        return state
+
+    @torch.no_grad()
+    def forward(self, token_ids: torch.Tensor, cu_seqlens: torch.Tensor, option_ids: torch.Tensor,
+                temperature: float = 1.0, prefix: PrefixState | None = None) -> torch.Tensor:
+        """token_ids [N] (packed prompts), cu_seqlens [B + 1] int32 (device), option_ids [n_opt]. Returns the
+        option probabilities [B, n_opt] float64 at each prompt's last position. ``prefix``: the prompts continue this one
+        (:meth:`prefill_prefix`), and token_ids holds only what follows it."""
+        c = self.cfg
+        cu = cu_seqlens.to(device=self.dev, dtype=torch.int32)
+        n = token_ids.numel()
+        lens = cu[1:] - cu[:-1]
+        max_len = int(lens.max())
+        start = 0 if prefix is None else prefix.length
+        if prefix is not None and len(prefix.keys) != c.layers:
+            raise ValueError(f"the prefix has {len(prefix.keys)} layers, the model {c.layers}")
+        self._cos_sin(start + max_len)
+        seq = torch.repeat_interleave(torch.arange(lens.numel(), device=self.dev), lens.long(), output_size=n)
+        pos = torch.arange(n, device=self.dev) - cu[:-1].long()[seq] + start
+        last = (cu[1:] - 1).long()
+        x = self.embed[token_ids.to(self.dev).long()] * self.normalizer
+        x = self._layers(x, pos, cu, max_len, last, prefix)
         if self.layer_log is not None:
             self.layer_log.append(x.clone())
         h = rms_norm(x, self.final_norm, c.eps)                      # [B, hidden]: the last rows only
