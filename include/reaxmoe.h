@@ -176,7 +176,8 @@ int reaxmoe_gelu_tanh_mul(const void* gate_up, int64_t rows, int32_t inter, void
  * out[row] = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max), s_j = scale * q . k_j over the keys seen (bf16 / fp16
  * products, fp32 sums; the weights exp(s_j - max) enter the second product rounded to the operands' type), and lse[row] =
  * max + log(sum). A row that sees no key gets out 0 and lse -inf. Keys that a row does not see do not change it, whatever
- * their values (infinities and NaN included). Query head h reads KV head h / (q_heads / kv_heads). Rows of q at and behind
+ * their values (infinities and NaN included); an element with an infinity or NaN among the values that it does see is one
+ * of the two. Query head h reads KV head h / (q_heads / kv_heads). Rows of q at and behind
  * cu_q[seqs] are not written. Inference only: there is no backward. */
 enum { REAXMOE_BF16 = 0, REAXMOE_FP16 = 1 };
 

@@ -864,7 +864,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       while (again != 0u) {
         const int src = __ffs(again) - 1;
         again &= again - 1u;
-        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src));
+        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src), false);
       }
     }
   }
@@ -924,10 +924,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
     acc[i] = none ? 0.0f : acc[i] * inv;
     bad |= !(fabsf(acc[i]) < INFINITY);
   }
-  if (__any_sync(0xffffffffu, bad) && l == l) {
-    row_by_warp<D, BF>(p.a, tok, head);
-    return;
-  }
   uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride;
   if constexpr (W == 2) {
     reinterpret_cast<uint32_t*>(out)[lane] = pack2<BF>(acc[0], acc[1]);
@@ -939,6 +935,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   }
   if (p.a.lse != nullptr && lane == 0)
     p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
+  __syncwarp();
+  if (__any_sync(0xffffffffu, bad) && l == l) row_by_warp<D, BF>(p.a, tok, head, false);
 }
 
 // Row tiles, parts of the keys, and the workspace: counter, partial maxima and sums, partial outputs (of pair_kernel, of

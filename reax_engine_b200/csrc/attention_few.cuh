@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewLayout<D>::BLOCKS) few_kern
   using L = FewLayout<D>;
   constexpr float THR = BF ? 64.0f : 11.0f;       // as in pair_kernel
   constexpr float SHIFT = BF ? 0.0f : 4.0f;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(smem) + warp * L::SLOTS * L::SLOT;
   const int ntok = min(__ldg(p.a.cu_q + p.a.seqs), (int)p.a.q_tokens);
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
   const int q0 = max(__ldg(p.a.cu_q + b), 0), q1 = min(sq.q_end, ntok);
   const int kvh = head / p.group, row = (tok - q0) * p.group + head - kvh * p.group;
   if (q1 - q0 > FEW_ROWS || (q1 - q0) * p.group > FEW_ROWS || tok >= q1) {
-    if (warp == 0) row_by_warp<D, BF>(p.a, tok, head);
+    if (warp == 0) row_by_warp<D, BF>(p.a, tok, head, true);
     return;
   }
   const int ke = sq.ks + sq.all - (int)p.a.prefix;
@@ -412,14 +412,12 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
     bad |= !(fabsf(y0) < INFINITY) || !(fabsf(y1) < INFINITY);
     packed[x / 2] = pack2<BF>(y0, y1);
   }
-  if (__any_sync(0xffffffffu, bad) && l == l) {          // a value that the row does not see (pair_kernel)
-    row_by_warp<D, BF>(p.a, tok, head);
-    return;
-  }
 #pragma unroll
   for (int x = 0; x < W / 2; ++x) out[lane + x * 32] = packed[x];
   if (p.a.lse != nullptr && lane == 0)
     p.a.lse[(int64_t)tok * p.a.q_heads + head] = none ? -INFINITY : (m - SHIFT + __log2f(l)) * 0.6931471805599453f;
+  __syncwarp();
+  if (__any_sync(0xffffffffu, bad) && l == l) row_by_warp<D, BF>(p.a, tok, head, false);     // (pair_kernel)
 }
 
 }  // namespace attn

@@ -91,57 +91,103 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One row by one warp, lane l holding elements [l D/32, (l+1) D/32): scores in fp32, running maximum and sum, key by key. It
-// reads the keys that the row sees and no others, which the tensor-core kernel cannot do where a tile of keys ends inside
-// what a row sees: there a masked key has weight 0, and 0 x (an infinity or NaN of its value) would be NaN.
+// One row by one warp, 32 keys at a time: lane = key for the scores, lane l = elements [l D/32, (l+1) D/32) for the sums. It
+// reads the keys that the row sees and no others, which tiles of keys cannot: there a key that a row does not see has weight
+// 0, and 0 x (an infinity or NaN of its value) is NaN.
+// all: the whole row; else only those elements of it whose value in `out` (already written) is not finite. These are done again
+// until none of them can become finite any more: then the values that are not finite are of keys that the row does see, and
+// `out` stays as it is (an infinity in a key that many rows see would take minutes otherwise).
 template <int D, bool BF>
-__device__ __forceinline__ void row_by_warp(const reaxmoe_attention_args& a, int t, int head) {
+__device__ __forceinline__ void row_by_warp(const reaxmoe_attention_args& a, int t, int head, bool all) {
   constexpr int W = D / 64;                      // 32-bit words per lane
   const int lane = threadIdx.x & 31;
   const int kvh = head / (a.q_heads / a.kv_heads);
   const RowKeys rk = row_keys(a, t);
-  auto load = [&](const void* base, int64_t row, int64_t stride, int64_t hs, int h, float2 (&f)[W]) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(base) + row * stride + h * hs) + lane * W;
+  uint32_t* po = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride + head * a.out_head_stride) + lane * W;
+  const uint4* pq = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (int64_t)t * a.q_stride + head * a.q_head_stride);
+  bool again[2 * W];
+  float acc[2 * W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) f[i] = unpack2<BF>(__ldg(p + i));
-  };
-  float2 q[W], acc[W];
-  load(a.q, t, a.q_stride, a.q_head_stride, head, q);
-#pragma unroll
-  for (int i = 0; i < W; ++i) acc[i] = make_float2(0.0f, 0.0f);
+  for (int i = 0; i < W; ++i) {
+    float2 v = make_float2(NAN, NAN);
+    if (!all) v = unpack2<BF>(*reinterpret_cast<volatile uint32_t*>(po + i));
+    again[2 * i] = !(fabsf(v.x) < INFINITY);
+    again[2 * i + 1] = !(fabsf(v.y) < INFINITY);
+    acc[2 * i] = acc[2 * i + 1] = 0.0f;
+  }
   const float c = a.scale * 1.4426950408889634f;  // scores in units of log2
   float m = -INFINITY, l = 0.0f;
-  auto keys = [&](const void* kb, int64_t ks, int64_t khs, const void* vb, int64_t vs, int64_t vhs, int lo, int hi) {
 #pragma unroll 1
-    for (int j = lo; j < hi; ++j) {
-      float2 k[W], v[W];
-      load(kb, j, ks, khs, kvh, k);
-      load(vb, j, vs, vhs, kvh, v);
-      float s = 0.0f;
+  for (int part = 0; part < 2; ++part) {
+    const uint16_t* kb = static_cast<const uint16_t*>(part == 0 ? a.prefix_k : a.k) + kvh * (part == 0 ? a.prefix_k_head_stride : a.k_head_stride);
+    const uint16_t* vb = static_cast<const uint16_t*>(part == 0 ? a.prefix_v : a.v) + kvh * (part == 0 ? a.prefix_v_head_stride : a.v_head_stride);
+    const int64_t ks = part == 0 ? a.prefix_k_stride : a.k_stride, vs = part == 0 ? a.prefix_v_stride : a.v_stride;
+    const int lo = part == 0 ? rk.p_lo : rk.k_lo, hi = part == 0 ? rk.p_hi : rk.k_hi;
+#pragma unroll 1
+    for (int j0 = lo; j0 < hi; j0 += 32) {
+      const int n = min(32, hi - j0);
+      float w;
+      {
+        float s = -INFINITY;
+        if (lane < n) {
+          const uint4* pk = reinterpret_cast<const uint4*>(kb + (int64_t)(j0 + lane) * ks);
+          s = 0.0f;
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 q4 = __ldg(pq + i), k4 = __ldg(pk + i);
+            const uint32_t qw[4] = {q4.x, q4.y, q4.z, q4.w}, kw[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-      for (int i = 0; i < W; ++i) s = fmaf(q[i].x, k[i].x, fmaf(q[i].y, k[i].y, s));
+            for (int e = 0; e < 4; ++e) {
+              const float2 qf = unpack2<BF>(qw[e]), kf = unpack2<BF>(kw[e]);
+              s = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, s));
+            }
+          }
+          s *= c;
+        }
+        float top = s;                            // NaN where a score is
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      s *= c;
-      // a NaN score stays one: fmaxf would drop it
-      const float mn = (s != s) ? s : fmaxf(m, s);
-      const float f = m == mn ? 1.0f : exp2f(m - mn);
-      const float p = s == mn && fabsf(s) != INFINITY ? 1.0f : exp2f(s - mn);
-      m = mn;
-      l = l * f + p;
+        for (int o = 16; o > 0; o >>= 1) {
+          const float x = __shfl_xor_sync(0xffffffffu, top, o);
+          top = (top != top || x != x) ? NAN : fmaxf(top, x);
+        }
+        const float mn = (top != top || m != m) ? NAN : fmaxf(m, top);
+        const float base = mn == -INFINITY ? 0.0f : mn, f = m == mn ? 1.0f : exp2f(m - base);
+        w = lane < n ? exp2f(s - base) : 0.0f;
+        float sum = w;
 #pragma unroll
-      for (int i = 0; i < W; ++i) acc[i] = make_float2(fmaf(acc[i].x, f, p * v[i].x), fmaf(acc[i].y, f, p * v[i].y));
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        m = mn;
+        l = l * f + sum;
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) acc[i] *= f;
+      }
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const uint32_t* pv = reinterpret_cast<const uint32_t*>(vb + (int64_t)(j0 + j) * vs) + lane * W;
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float2 v = unpack2<BF>(__ldg(pv + i));
+          acc[2 * i] = fmaf(wj, v.x, acc[2 * i]);
+          acc[2 * i + 1] = fmaf(wj, v.y, acc[2 * i + 1]);
+        }
+      }
+      if (!all) {
+        bool over = true;
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) over &= !again[i] || !(fabsf(acc[i]) < INFINITY);
+        if (__all_sync(0xffffffffu, over)) return;
+      }
     }
-  };
-  keys(a.prefix_k, a.prefix_k_stride, a.prefix_k_head_stride, a.prefix_v, a.prefix_v_stride, a.prefix_v_head_stride, rk.p_lo,
-       rk.p_hi);
-  keys(a.k, a.k_stride, a.k_head_stride, a.v, a.v_stride, a.v_head_stride, rk.k_lo, rk.k_hi);
+  }
   const bool none = rk.p_lo >= rk.p_hi && rk.k_lo >= rk.k_hi;
   const float inv = none ? 0.0f : 1.0f / l;
-  uint32_t* po = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride + head * a.out_head_stride) + lane * W;
 #pragma unroll
-  for (int i = 0; i < W; ++i) po[i] = pack2<BF>(acc[i].x * inv, acc[i].y * inv);
-  if (a.lse != nullptr && lane == 0)
+  for (int i = 0; i < W; ++i) {
+    const float2 old = all ? make_float2(0.0f, 0.0f) : unpack2<BF>(*reinterpret_cast<volatile uint32_t*>(po + i));
+    po[i] = pack2<BF>(again[2 * i] ? acc[2 * i] * inv : old.x, again[2 * i + 1] ? acc[2 * i + 1] * inv : old.y);
+  }
+  if (all && a.lse != nullptr && lane == 0)
     a.lse[(int64_t)t * a.q_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
