@@ -333,6 +333,70 @@ def test_new_lengths_in_a_captured_call():
         check(out, reference(q, k, v, lens, lens, 64 ** -0.5))
 
 
+def test_no_keys_at_all():
+    import reax_engine_b200 as R
+    q, k, v, pk, pv = tensors(5, 0, 4, 2, 128, "bf16", 1, prefix=3)
+    c, ck = dev([0, 2, 5]), dev([0, 0, 0])
+    o, lse = R.prompt_attention(q, k, v, c, ck, return_lse=True)
+    assert (o == 0).all() and (lse == -torch.inf).all()
+    o, lse = R.shared_prefix_attention(q, k, v, pk[:0], pv[:0], c, ck, return_lse=True)
+    assert (o == 0).all() and (lse == -torch.inf).all()
+    o, lse = R.shared_prefix_attention(q, k, v, pk, pv, c, ck, causal=False, return_lse=True)
+    check(o, reference(q, k, v, [0, 2, 5], [0, 0, 0], 128 ** -0.5, causal=False, prefix_k=pk, prefix_v=pv), lse)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_offsets_past_32_bits(rows):
+    """Keys behind the 2^31st element of their buffer (whose rest holds whatever memory held), query and output rows 2^22 elements
+    apart."""
+    import reax_engine_b200 as R
+    n, hk, d, tail = 1_100_000, 8, 256, 300
+    k, v = (torch.empty(n, hk, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q0, k0, v0, _, _ = tensors(rows, tail, 16, hk, d, "bf16", 3)
+    k[-tail:], v[-tail:] = k0, v0
+    span = (600 - 1) * (1 << 22) + 16 * d
+    q, out = (torch.empty(span, dtype=torch.bfloat16, device="cuda").as_strided((600, 16, d), (1 << 22, d, 1)) for _ in range(2))
+    q[-rows:] = q0
+    ck = [0, n - tail, n]
+    o, lse = R.prompt_attention(q[600 - rows:], k, v, dev([0, 0, rows]), dev(ck), out=out[600 - rows:], return_lse=True)
+    check(o, reference(q0, k0, v0, [0, rows], [0, tail], d ** -0.5), lse)
+
+
+def test_first_call_of_a_process_under_capture():
+    code = (
+        "import torch, reax_engine_b200 as R\n"
+        "t = [torch.randn(30, h, 64, device='cuda').bfloat16() for h in (4, 2, 2)]\n"
+        "c = torch.tensor([0, 10, 30], dtype=torch.int32, device='cuda')\n"
+        "torch.cuda.synchronize()\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    o = R.prompt_attention(*t, c)\n"
+        "g.replay()\n"
+        "torch.cuda.synchronize()\n"
+        "assert torch.equal(o, R.prompt_attention(*t, c)) and o.float().abs().sum() > 0\n")
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_sm_budget():
+    """Fewer SMs, other parts of the keys: the same answers, and workspaces of the new sizes."""
+    import reax_engine_b200 as R
+    q, k, v, pk, pv = tensors(3, 3000, 4, 1, 64, "bf16", 4, prefix=1000)
+    cq, ck = [0, 1, 2, 3], [0, 1500, 1503, 3000]
+    ref = reference(q, k, v, cq, ck, 64 ** -0.5, prefix_k=pk, prefix_v=pv)
+    try:
+        for sms in (1, 20, 0, 75):
+            R.set_sm_budget(sms)
+            check(R.shared_prefix_attention(q, k, v, pk, pv, dev(cq), dev(ck)), ref)
+            check(R.prompt_attention(q, k, v, dev(cq), dev(ck)), reference(q, k, v, cq, ck, 64 ** -0.5))
+    finally:
+        R.set_sm_budget(0)
+
+
 def test_workspace_and_status():
     import reax_engine_b200 as R
     from reax_engine_b200 import _lib as L
