@@ -432,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         it.first = sequence_at(p.a, it.b0);
         int plo = INT_MAX, phi = 0, klo = INT_MAX, khi = 0;
         unsigned sum = 0;
-#pragma unroll 1
+#pragma unroll 4
         for (int b = it.b0 + lane; b <= it.b1; b += 32) {
           const int f = max(t0, __ldg(p.a.cu_q + b)), l = min(t1, __ldg(p.a.cu_q + b + 1)) - 1;
           if (f > l) continue;
