@@ -20,8 +20,8 @@ from .moe import _require_cuda
 
 _DTYPES = {torch.bfloat16: L.BF16, torch.float16: L.FP16}
 
-# What the checks of a call found for one set of shapes, strides, types and options: the argument block without its pointers
-# and the workspace's size. Emptied when the SM budget changes, on which the size depends.
+# What the checks of a call found for one set of shapes, strides, types and options (of tensors that need no copy): the argument
+# block without its pointers and the workspace's size. Emptied when the SM budget changes, on which the size depends.
 _checked: dict = {}
 _unused: dict = {}        # device -> the workspace of calls that use none
 _CHECKED_MAX = 4096
@@ -55,6 +55,19 @@ def _lengths(cu: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
     return cu.to(torch.int32).contiguous()
 
 
+def _output(out: torch.Tensor, q: torch.Tensor, inputs) -> torch.Tensor:
+    """What the kernels write for the caller's `out`: itself, or a copy where its rows cannot be addressed."""
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must have the shape, dtype and device of q")
+    if any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in inputs):
+        raise ValueError("out must not share its storage with an input")
+    if out.ndim != 3:
+        raise ValueError("q must be [tokens, heads, head_dim]")
+    s0, s1, s2 = out.stride()
+    ok = s2 == 1 and out.data_ptr() % 16 == 0 and s0 % 8 == 0 and s1 % 8 == 0
+    return out if ok else out.clone(memory_format=torch.contiguous_format)
+
+
 def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window):
     """The argument block of these tensors without its pointers, and the workspace's size."""
     ts = [("q", q), ("k", k), ("v", v)] + ([] if prefix_k is None else [("prefix_k", prefix_k), ("prefix_v", prefix_v)])
@@ -85,50 +98,58 @@ def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window
     return bytes(args), need
 
 
+def _aligned(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 == 0
+
+
 def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out, workspace, status):
-    inputs = (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v)
-    for t in inputs:
-        if not t.is_cuda:
-            _require_cuda(t)
-        if t.ndim != 3:
-            raise ValueError("q, k, v and the prefix must be [tokens, heads, head_dim]")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
     device = q.device
+    if device.type != "cuda":
+        _require_cuda(q)
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out,
                               workspace, status)
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (prefix_k is not None and (
+            prefix_k.requires_grad or prefix_v.requires_grad))) and torch.is_grad_enabled():
+        raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
     cu_q = _lengths(cu_seqlens, "cu_seqlens", device)
     cu_k = cu_q if cu_seqlens_k is None else _lengths(cu_seqlens_k, "cu_seqlens_k", device)
+    shape = q.shape
     if out is None:
-        dst = torch.empty(q.shape, dtype=q.dtype, device=device)
+        if len(shape) != 3:
+            raise ValueError("q must be [tokens, heads, head_dim]")
+        dst = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=q.dtype, device=device)
     else:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
-            raise ValueError("out must have the shape, dtype and device of q")
-        if any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in inputs):
-            raise ValueError("out must not share its storage with an input")
-        s0, s1, s2 = out.stride()
-        ok = s2 == 1 and out.data_ptr() % 16 == 0 and s0 % 8 == 0 and s1 % 8 == 0
-        dst = out if ok else out.clone(memory_format=torch.contiguous_format)
+        dst = _output(out, q, (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v))
     if status is not None and (status.dtype != torch.int32 or status.device != device or status.numel() < 1):
         raise ValueError("status must be an int32 tensor on the device of q")
-    q, k, v = _heads(q), _heads(k), _heads(v)
-    if prefix_k is not None:
-        prefix_k, prefix_v = _heads(prefix_k), _heads(prefix_v)
-    key = (device, q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, dst.stride(),
-           cu_q.shape, cu_k.shape, scale, causal, window, k.device, v.device)
+    if scale is not None:
+        scale = float(scale)
+    key = (device, shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+           dst.stride(), cu_q.shape, cu_k.shape, scale, causal, window)
+    aligned = _aligned(q) and _aligned(k) and _aligned(v)
     if prefix_k is not None:
         key += (prefix_k.shape, prefix_k.stride(), prefix_k.dtype, prefix_k.device, prefix_v.shape, prefix_v.stride(),
                 prefix_v.dtype, prefix_v.device)
-    found = _checked.get(key)
+        aligned = aligned and _aligned(prefix_k) and _aligned(prefix_v)
+    found = _checked.get(key) if aligned else None
     if found is None:
+        for t in (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v):
+            _require_cuda(t)
+            if t.ndim != 3:
+                raise ValueError("q, k, v and the prefix must be [tokens, heads, head_dim]")
+        as_they_are = all(map(_readable, (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v)))
+        q, k, v = _heads(q), _heads(k), _heads(v)
+        if prefix_k is not None:
+            prefix_k, prefix_v = _heads(prefix_k), _heads(prefix_v)
         found = _check(q, k, v, prefix_k, prefix_v, cu_q.numel(), cu_k.numel(), dst, scale, causal, window)
-        if len(_checked) >= _CHECKED_MAX:
-            _checked.clear()
-        _checked[key] = found
+        if as_they_are:
+            if len(_checked) >= _CHECKED_MAX:
+                _checked.clear()
+            _checked[key] = found
     block, need = found
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    lse = torch.empty_strided(shape[:2], (shape[1], 1), dtype=torch.float32, device=device) if return_lse else None
     if workspace is None:
         if need <= _UNUSED:
             workspace = _unused.get(device)
