@@ -973,9 +973,10 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   pl.items = (int)items;
   pl.pairs = (int)(items < pairs ? items : pairs);
   // units of few_kernel, of at least 64 keys: with few sequences one for every warp of the device (each sequence may have one
-  // more than its share), else about three, so that the ends of sequences even out
+  // more than its share), else about five, so that the ends of sequences even out (64 sequences of about 2304 keys, D = 256: 252
+  // us with two a warp, 241 with three, 236 with five, 235 with eight, whose joining costs more at D = 128)
   const int64_t warps = ceil_div64((int64_t)num_sms * FEW_WARPS, a.kv_heads);       // for each KV head
-  int64_t chunk = ceil_div64(a.k_tokens, warps >= 8 * (int64_t)a.seqs ? warps - a.seqs : 3 * warps);
+  int64_t chunk = ceil_div64(a.k_tokens, warps >= 8 * (int64_t)a.seqs ? warps - a.seqs : 5 * warps);
   chunk = chunk < 64 ? 64 : ceil_div64(chunk, 16) * 16;
   pl.chunk = (int)chunk;
   pl.units = pl.few ? (int)(ceil_div64(a.k_tokens, chunk) + a.seqs) : 0;
