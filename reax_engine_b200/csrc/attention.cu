@@ -49,6 +49,18 @@ constexpr int THREADS = (OUT_WARP0 + OUT_WARPS) * 32;
 constexpr int REGS_SOFTMAX = 168, REGS_CONTROL = 64, REGS_OUT = 112;
 static_assert(2 * REGS_SOFTMAX + REGS_CONTROL + REGS_OUT == 4 * 128 && THREADS == 512, "register shares");
 
+struct ItemInfo {
+  int row0;          // first row of the pair's tile; -1: no more items
+  int b0, b1;        // first and last sequence that has rows in it
+  Sequence first;    // the first
+  int head, part;    // KV head, part of the keys
+  int p_lo, p_hi;    // prefix keys of this part
+  int o_lo, o_hi;    // own keys of this part
+  int gap;           // keys that no row sees lie between those of two sequences
+  int tiles;         // of 128 keys each
+};
+
+// Shared memory: Q, the ring of K and V slots, words, barriers (8 bytes each, by index), and what follows them.
 template <int D>
 struct Layout {
   static constexpr int NB = D == 256 ? 2 : 3;               // S buffers; TMEM columns: S0, S1, (S2,) O
@@ -59,19 +71,31 @@ struct Layout {
   static constexpr int ring = Q_BYTES;
   static constexpr int words = ring + SLOTS * SLOT;         // [2][2][ROWS]: what the column halves of a row exchange, by parity
   static constexpr int bars = words + 4 * ROWS * 4;
+  enum Bar {
+    FULL = 0,                          // [SLOTS] (leader's) both CTAs' halves landed (tx)
+    EMPTY = FULL + SLOTS,              // [SLOTS] the slot's MMAs are done (commit to both CTAs)
+    S_FULL = EMPTY + SLOTS,            // [NB] S is in TMEM (commit to both)
+    P_FULL = S_FULL + NB,              // [NB] (leader's) P is in TMEM (16 warps of the pair)
+    PV_DONE = P_FULL + NB,             // [2] a tile's P V is in O (commit to both)
+    O_FULL = PV_DONE + 2,              // the item's O is complete (commit to both)
+    O_EMPTY = O_FULL + 1,              // (leader's) O has been read out (8 warps of the pair)
+    Q_FULL = O_EMPTY + 1,              // (leader's) both CTAs' Q rows landed (tx)
+    Q_EMPTY = Q_FULL + 1,              // the item's Q K^T are done (commit to both)
+    INFO_FULL = Q_EMPTY + 1,           // [2] item info is there
+    INFO_EMPTY = INFO_FULL + 2,        // [2] item info has been read (producer, MMA, softmax and output warps)
+    ITEM_FULL = INFO_EMPTY + 2,        // the next item's number arrived (tx)
+    ITEM_FREE = ITEM_FULL + 1,         // (leader's) both CTAs took it
+    L_FULL = ITEM_FREE + 1,            // the item's factors 1 / sum are in shared memory (4 softmax warps)
+    L_EMPTY = L_FULL + 1,              // they have been read (4 output warps)
+    DRAIN = L_EMPTY + 1,               // every MMA is done
+    BARS = DRAIN + 1
+  };
+  static constexpr int inv_l = bars + BARS * 8;             // [ROWS] floats
+  static constexpr int info = (inv_l + ROWS * 4 + 7) / 8 * 8;      // [2] ItemInfo
+  static constexpr int state = info + 2 * (int)sizeof(ItemInfo);   // next_item, tmem_holder, abort_flag
   static constexpr int total = bars + 1024;
+  static_assert(alignof(ItemInfo) <= 8 && state + 3 * 4 <= total, "what follows the barriers");
   static_assert(total <= 232448, "shared memory");
-};
-
-struct ItemInfo {
-  int row0;          // first row of the pair's tile; -1: no more items
-  int b0, b1;        // first and last sequence that has rows in it
-  Sequence first;    // the first
-  int head, part;    // KV head, part of the keys
-  int p_lo, p_hi;    // prefix keys of this part
-  int o_lo, o_hi;    // own keys of this part
-  int gap;           // keys that no row sees lie between those of two sequences
-  int tiles;         // of 128 keys each
 };
 
 struct Params {
@@ -169,25 +193,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   constexpr float SHIFT = BF ? 0.0f : 4.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::bars);
-  uint64_t* full = bars;               // [NS] (leader's) both CTAs' halves landed (tx)
-  uint64_t* empty = full + NS;         // [NS] the slot's MMAs are done (commit to both CTAs)
-  uint64_t* s_full = empty + NS;       // [NB] S is in TMEM (commit to both)
-  uint64_t* p_full = s_full + NB;      // [NB] (leader's) P is in TMEM (16 warps of the pair)
-  uint64_t* pv_done = p_full + NB;     // [2] a tile's P V is in O (commit to both)
-  uint64_t* o_full = pv_done + 2;      // the item's O is complete (commit to both)
-  uint64_t* o_empty = o_full + 1;      // (leader's) O has been read out (8 warps of the pair)
-  uint64_t* q_full = o_empty + 1;      // (leader's) both CTAs' Q rows landed (tx)
-  uint64_t* q_empty = q_full + 1;      // the item's Q K^T are done (commit to both)
-  uint64_t* info_full = q_empty + 1;   // [2] item info is there
-  uint64_t* info_empty = info_full + 2;// [2] item info has been read (producer, MMA, softmax and output warps)
-  uint64_t* item_full = info_empty + 2;// the next item's number arrived (tx)
-  uint64_t* item_free = item_full + 1; // (leader's) both CTAs took it
-  uint64_t* l_full = item_free + 1;    // the item's factors 1 / sum are in shared memory (4 softmax warps)
-  uint64_t* l_empty = l_full + 1;      // they have been read (4 output warps)
-  uint64_t* drainb = l_empty + 1;
-  float* inv_l = reinterpret_cast<float*>(drainb + 1);                  // [ROWS]
-  ItemInfo* info = reinterpret_cast<ItemInfo*>(inv_l + ROWS);           // [2]
-  uint32_t* next_item = reinterpret_cast<uint32_t*>(info + 2);
+  uint64_t *full = bars + L::FULL, *empty = bars + L::EMPTY, *s_full = bars + L::S_FULL, *p_full = bars + L::P_FULL;
+  uint64_t *pv_done = bars + L::PV_DONE, *o_full = bars + L::O_FULL, *o_empty = bars + L::O_EMPTY, *q_full = bars + L::Q_FULL;
+  uint64_t *q_empty = bars + L::Q_EMPTY, *info_full = bars + L::INFO_FULL, *info_empty = bars + L::INFO_EMPTY;
+  uint64_t *item_full = bars + L::ITEM_FULL, *item_free = bars + L::ITEM_FREE, *l_full = bars + L::L_FULL;
+  uint64_t *l_empty = bars + L::L_EMPTY, *drainb = bars + L::DRAIN;
+  float* inv_l = reinterpret_cast<float*>(smem + L::inv_l);
+  ItemInfo* info = reinterpret_cast<ItemInfo*>(smem + L::info);
+  uint32_t* next_item = reinterpret_cast<uint32_t*>(smem + L::state);
   uint32_t* tmem_holder = next_item + 1;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
