@@ -312,7 +312,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           if (ok && j >= AHEAD) ok = fill(true, start[AHEAD], pre[AHEAD], it.head);
         }
       }
-      // let the last loads land before the CTA may exit (only matters after an abort)
+      // let the last loads that the leader knows of land before the CTAs may exit (only matters after an abort)
       if (rank == 0)
 #pragma unroll 1
         for (int f = n - 1; f >= 0 && f >= n - NS; --f) wait_drain(smem_u32(&full[f % NS]), (uint32_t)(f / NS) & 1u);
@@ -516,6 +516,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       __syncwarp();
       ++items;
     }
+    if (rank == 0 && lane == 0 && items > 0) wait_drain(smem_u32(q_full), (uint32_t)(items - 1) & 1u);     // as in warp 8
   }
   } else if (warp < SM_WARPS) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
@@ -881,6 +882,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       }
     }
   }
+  // After an abort the other CTA may have loads under way that count on the leader's barriers without the leader's knowledge,
+  // and item numbers and arrivals may be on their way to the other CTA. Whatever a warp started before it comes here has the
+  // time to land: the warp that set the flag comes here after it.
+  if (*abort_flag != 0) settle();
   tc_fence_before();
   __syncwarp();
   cluster_sync();                       // neither CTA's shared memory nor TMEM is in use any more

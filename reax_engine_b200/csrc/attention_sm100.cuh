@@ -44,6 +44,12 @@ __device__ __forceinline__ void st_async_u32(uint32_t dst, uint32_t v, uint32_t 
                : "memory");
 }
 
+// 2 ms, in which copies under way land that no barrier of this CTA counts (they take some microseconds).
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = globaltimer();
+  while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+}
+
 // box of a [tokens, heads, dim] tensor into this CTA's shared memory; the bytes count on `bar` (shared::cluster address), which
 // may be the pair's other CTA's
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, int z) {
