@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
   const Sequence sq = sequence_at(p.a, b);
   const int q0 = max(__ldg(p.a.cu_q + b), 0), q1 = min(sq.q_end, ntok);
   const int kvh = head / p.group, row = (tok - q0) * p.group + head - kvh * p.group;
-  if (q1 - q0 > FEW_ROWS || (q1 - q0) * p.group > FEW_ROWS || tok >= q1) {
+  // too many rows for few_kernel (or, where the lengths do not rise from 0, a row outside its sequence, which has no place there)
+  if (q1 - q0 > FEW_ROWS || (q1 - q0) * p.group > FEW_ROWS || tok < q0 || tok >= q1) {
     if (warp == 0) row_by_warp<D, BF>(p.a, tok, head, true);
     return;
   }

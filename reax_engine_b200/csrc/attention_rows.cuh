@@ -43,7 +43,8 @@ __device__ __forceinline__ int sequence_by_warp(const reaxmoe_attention_args& a,
 }
 
 // A sequence: its first own key, prefix and own keys together, and the token behind its last query row. The cumulative lengths
-// are cut to the tensors, so that no value of theirs makes a later access leave them.
+// are cut to the tensors here and a row's distance to its sequence's end to at least 1 below, so that no value of theirs (a first
+// one that is not 0, falling or negative ones) makes a later access leave the tensors.
 struct Sequence {
   int ks, all, q_end;
 };
@@ -52,14 +53,14 @@ __device__ __forceinline__ Sequence sequence_at(const reaxmoe_attention_args& a,
   Sequence s;
   s.ks = min(max(__ldg(a.cu_k + b), 0), kt);
   s.all = (int)a.prefix + min(max(__ldg(a.cu_k + b + 1), s.ks), kt) - s.ks;
-  s.q_end = __ldg(a.cu_q + b + 1);
+  s.q_end = min(max(__ldg(a.cu_q + b + 1), 0), (int)a.q_tokens);
   return s;
 }
 
 // Keys that its query token t sees.
 __device__ __forceinline__ RowKeys row_keys_in(const reaxmoe_attention_args& a, const Sequence& s, int t) {
   const int P = (int)a.prefix;
-  const int pos = s.all - (s.q_end - t);                         // prefix + n - m + i
+  const int pos = s.all - max(s.q_end - t, 1);                   // prefix + n - m + i
   const int hi = a.causal ? min(max(pos, -1) + 1, s.all) : s.all;
   const int lo = a.window > 0 && pos >= a.window ? min(pos - a.window + 1, hi) : 0;
   RowKeys r;

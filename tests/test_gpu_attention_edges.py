@@ -1,0 +1,25 @@
+"""Calls of prompt_attention and shared_prefix_attention at their edges. Tolerances: those of test_gpu_attention."""
+import pytest
+import torch
+
+from test_gpu_attention import check, cu, dev, reference, tensors
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d,prefix,keys", [(64, 0, 300), (128, 0, 300), (64, 150, 5000), (256, 150, 300)])
+def test_lengths_that_do_not_rise_from_zero(d, prefix, keys):
+    """Rows before the first sequence's, and lengths that fall: outside the contract, their values are anything, but rows of
+    sequences that are well-formed are right, and so is the next call."""
+    import reax_engine_b200 as R
+    q, k, v, pk, pv = tensors(12, keys, 4, 2, d, "bf16", d, prefix=prefix)
+    call = lambda cq, ck: (R.shared_prefix_attention(q, k, v, pk, pv, dev(cq), dev(ck)) if prefix  # noqa: E731
+                           else R.prompt_attention(q, k, v, dev(cq), dev(ck)))
+    ck = [0, 40, 100, keys - 20] + [keys] * 10
+    cq = [9, 10, 11, 12] + [12] * 10
+    ref = reference(q, k, v, cq, ck, d ** -0.5, prefix_k=pk, prefix_v=pv)
+    check(call(cq, ck)[9:], [x[9:] for x in ref])
+    for bad in ([7, 3, 9, 1, 12] + [12] * 9, [2 ** 31 - 1] * 13 + [12], [-2 ** 31] * 13 + [12], [0] * 13 + [2 ** 31 - 1]):
+        call(bad, ck)
+        call(cq, [keys - 1, -5, 2 ** 31 - 1, 3] + [-2 ** 31, 7] * 5)
+    check(call(cq, ck)[9:], [x[9:] for x in ref])
