@@ -146,10 +146,12 @@ def gelu_tanh_mul(gu: torch.Tensor) -> torch.Tensor:
 @dataclass
 class PrefixState:
     """A prefix that prompts continue: its keys and values of every layer, [length, kv_heads, head_dim] bf16 (after the norms
-    and RoPE at positions 0 .. length - 1)."""
+    and RoPE at positions 0 .. length - 1), and the last layer's output of its last token, [1, hidden], which answers for a
+    prompt that adds nothing."""
     length: int
     keys: list
     values: list
+    last: torch.Tensor | None = None
 
 
 class DecisionModel:
@@ -343,7 +345,7 @@ class DecisionModel:
         pos = torch.arange(n, device=self.dev)
         cu = torch.tensor([0, n], dtype=torch.int32, device=self.dev)
         state = PrefixState(n, [], [])
-        self._layers(x, pos, cu, n, torch.tensor([n - 1], device=self.dev), keep=state)
+        state.last = self._layers(x, pos, cu, n, torch.tensor([n - 1], device=self.dev), keep=state)
         return state
 
     @torch.no_grad()
@@ -351,21 +353,34 @@ class DecisionModel:
                 temperature: float = 1.0, prefix: PrefixState | None = None) -> torch.Tensor:
         """token_ids [N] (packed prompts), cu_seqlens [B + 1] int32 (device), option_ids [n_opt]. Returns the
         option probabilities [B, n_opt] float64 at each prompt's last position. ``prefix``: the prompts continue this one
-        (:meth:`prefill_prefix`), and token_ids holds only what follows it."""
+        (:meth:`prefill_prefix`), and token_ids holds only what follows it; a prompt of no tokens is the prefix itself."""
         c = self.cfg
         cu = cu_seqlens.to(device=self.dev, dtype=torch.int32)
         n = token_ids.numel()
         lens = cu[1:] - cu[:-1]
-        max_len = int(lens.max())
+        max_len, min_len = torch.stack([lens.max(), lens.min()]).tolist()
         start = 0 if prefix is None else prefix.length
         if prefix is not None and len(prefix.keys) != c.layers:
             raise ValueError(f"the prefix has {len(prefix.keys)} layers, the model {c.layers}")
+        some = None                          # which prompts have tokens, where some continue the prefix with none
+        if prefix is not None and min_len < 1:
+            if prefix.last is None:
+                raise ValueError("a prompt of no tokens needs the prefix's last row (PrefixState.last)")
+            some = lens > 0
+            cu = torch.cat([cu[:1], cu[1:][some]])
+            lens = lens[some]
         self._cos_sin(start + max_len)
         seq = torch.repeat_interleave(torch.arange(lens.numel(), device=self.dev), lens.long(), output_size=n)
         pos = torch.arange(n, device=self.dev) - cu[:-1].long()[seq] + start
         last = (cu[1:] - 1).long()
-        x = self.embed[token_ids.to(self.dev).long()] * self.normalizer
-        x = self._layers(x, pos, cu, max_len, last, prefix)
+        if max_len > 0:
+            x = self.embed[token_ids.to(self.dev).long()] * self.normalizer
+            x = self._layers(x, pos, cu, max_len, last, prefix)
+        if some is not None:
+            rows = prefix.last.repeat(some.numel(), 1)
+            if max_len > 0:
+                rows[some] = x
+            x = rows
         if self.layer_log is not None:
             self.layer_log.append(x.clone())
         h = rms_norm(x, self.final_norm, c.eps)                      # [B, hidden]: the last rows only
