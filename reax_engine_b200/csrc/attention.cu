@@ -28,7 +28,8 @@
 //   warps 12..15  output: O from TMEM, divided by the sums, while the softmax warps are at the next item's first tiles
 // Items (row tile, KV head, part of the keys) are taken in order, the first by pair number, further ones from a counter.
 // With few rows an item's keys are split over several pairs, which leave partial sums that combine_kernel joins.
-// All waits are bounded (globaltimer); a timeout records REAXMOE_ERR_DEVICE_TIMEOUT and the CTA winds down.
+// All waits are bounded (globaltimer, from the last sign of life of those who do long work); a timeout records
+// REAXMOE_ERR_DEVICE_TIMEOUT and the CTA winds down.
 #include <atomic>
 #include <cstring>
 
@@ -92,9 +93,9 @@ struct Layout {
   };
   static constexpr int inv_l = bars + BARS * 8;             // [ROWS] floats
   static constexpr int info = (inv_l + ROWS * 4 + 7) / 8 * 8;      // [2] ItemInfo
-  static constexpr int state = info + 2 * (int)sizeof(ItemInfo);   // next_item, tmem_holder, abort_flag
+  static constexpr int state = info + 2 * (int)sizeof(ItemInfo);   // next_item, tmem_holder, abort_flag, beat
   static constexpr int total = bars + 1024;
-  static_assert(alignof(ItemInfo) <= 8 && state + 3 * 4 <= total, "what follows the barriers");
+  static_assert(alignof(ItemInfo) <= 8 && state + 4 * 4 <= total, "what follows the barriers");
   static_assert(total <= 232448, "shared memory");
 };
 
@@ -203,6 +204,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   uint32_t* next_item = reinterpret_cast<uint32_t*>(smem + L::state);
   uint32_t* tmem_holder = next_item + 1;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  volatile uint32_t* beat = tmem_holder + 2;     // changes with every slot filled and every 32 keys of a row done key by key
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -212,7 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     return;
   }
   auto wait1 = [&](uint64_t* bar, uint32_t parity) {
-    return wait_bounded(smem_u32(bar), parity & 1u, abort_flag, p.a.status, p.timeout_ns);
+    return wait_alive(smem_u32(bar), parity & 1u, abort_flag, beat, p.a.status, p.timeout_ns);
   };
   // every lane of a warp waits and all get the same answer
   auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait1(bar, parity)) != 0; };
@@ -241,6 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
     mbar_init(smem_u32(l_empty), OUT_WARPS);
     mbar_init(smem_u32(drainb), 1);
     *abort_flag = 0;
+    *beat = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = threadIdx.x; i < 4 * ROWS; i += THREADS) sts_volatile(smem_u32(smem + L::words) + i * 4, 1u);   // not the first use's
@@ -278,7 +281,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           for (int c = 0; c < D / 2 / W; ++c)
             tma_load_3d_pair(dst + c * (KT * W * 2), tm, bar, (int)rank * (D / 2) + c * W, head, start);
         }
-        ++n;
+        *beat = (uint32_t)++n;
         if (++s == NS) {
           s = 0;
           sphase ^= 1u;
@@ -566,10 +569,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       ++x_n;
       uint32_t v = lds_volatile(at);
       uint64_t t0 = 0;
+      uint32_t seen = 0;
 #pragma unroll 1
       for (uint32_t n = 1; !__all_sync(0xffffffffu, (v & 1u) == tag); ++n) {
         if ((n & 63u) == 0u) {
-          if (t0 == 0) t0 = globaltimer();
+          const uint32_t now = *beat;
+          if (t0 == 0 || now != seen) t0 = globaltimer();
+          seen = now;
           const bool late = globaltimer() - t0 > p.timeout_ns;
           if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
             if (late) set_status(p.a.status, REAXMOE_ERR_DEVICE_TIMEOUT);
@@ -878,7 +884,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       while (again != 0u) {
         const int src = __ffs(again) - 1;
         again &= again - 1u;
-        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src), false);
+        // (the other warps of both CTAs may have to wait for this one meanwhile)
+        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src), false, [&]() {
+          if (lane < 2) st_cluster_u32(map_to_rank(smem_u32(const_cast<uint32_t*>(beat)), (uint32_t)lane), (uint32_t)globaltimer());
+        });
       }
     }
   }

@@ -98,8 +98,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // all: the whole row; else only those elements of it whose value in `out` (already written) is not finite. These are done again
 // until none of them can become finite any more: then the values that are not finite are of keys that the row does see, and
 // `out` stays as it is (an infinity in a key that many rows see would take minutes otherwise).
-template <int D, bool BF>
-__device__ __forceinline__ void row_by_warp(const reaxmoe_attention_args& a, int t, int head, bool all) {
+// alive(): called by the whole warp every 32 keys.
+struct NoSign {
+  __device__ __forceinline__ void operator()() const {}
+};
+template <int D, bool BF, typename Alive = NoSign>
+__device__ __forceinline__ void row_by_warp(const reaxmoe_attention_args& a, int t, int head, bool all, Alive alive = Alive()) {
   constexpr int W = D / 64;                      // 32-bit words per lane
   const int lane = threadIdx.x & 31;
   const int kvh = head / (a.q_heads / a.kv_heads);
@@ -127,6 +131,7 @@ __device__ __forceinline__ void row_by_warp(const reaxmoe_attention_args& a, int
 #pragma unroll 1
     for (int j0 = lo; j0 < hi; j0 += 32) {
       const int n = min(32, hi - j0);
+      alive();
       float w;
       {
         float s = -INFINITY;

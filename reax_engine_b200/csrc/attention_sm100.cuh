@@ -44,6 +44,36 @@ __device__ __forceinline__ void st_async_u32(uint32_t dst, uint32_t v, uint32_t 
                : "memory");
 }
 
+// Bounded wait (sm100::wait_bounded) for work that may take long: the limit counts from the last sign of life in `beat`, a word of
+// this CTA that those who do long work change as they go (loads of key tiles, rows done key by key). A limit of 0 takes no signs:
+// whatever has to wait gives up.
+__device__ __forceinline__ bool wait_alive(uint32_t bar, uint32_t parity, volatile int* abort_flag, volatile uint32_t* beat,
+                                           int* status, unsigned long long timeout_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = globaltimer();
+  uint32_t seen = *beat;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 31u) == 0u) {
+      if (*abort_flag) return false;
+      if (globaltimer() - t0 > timeout_ns) {
+        const uint32_t now = *beat;
+        if (now == seen || timeout_ns == 0) {
+          *abort_flag = 1;
+          set_status(status, REAXMOE_ERR_DEVICE_TIMEOUT);
+          return false;
+        }
+        seen = now;
+        t0 = globaltimer();
+      }
+    }
+  }
+}
+// a sign of life in both CTAs of the pair (addresses from map_to_rank)
+__device__ __forceinline__ void st_cluster_u32(uint32_t dst, uint32_t v) {
+  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+}
+
 // 2 ms, in which copies under way land that no barrier of this CTA counts (they take some microseconds).
 __device__ __forceinline__ void settle() {
   const uint64_t t0 = globaltimer();

@@ -3,7 +3,7 @@ works on."""
 import pytest
 import torch
 
-from test_gpu_attention import cu, dev, tensors
+from test_gpu_attention import check, cu, dev, reference, tensors
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,33 @@ def test_waits_that_may_not_last(monkeypatch, lens, d, dtype):
             assert torch.equal(got, want)
         status.zero_()
         assert torch.equal(R.shared_prefix_attention(q, k, v, pk, pv, c, status=status), want) and int(status) == 0
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_done_key_by_key_do_not_run_out_the_waits_for_them(monkeypatch, d):
+    """One pair of CTAs, several items, and in each a last key whose value is NaN, which only the last row sees: the other rows of
+    its tile are done again one key after another, which takes far longer than the waits may last without a sign of life."""
+    import reax_engine_b200 as R
+    m, n, h = 128, 12000, 4
+    q, k, v, _, _ = tensors(m, n, h, h, d, "bf16", d)
+    v[-1] = float("nan")
+    c, ck = dev([0, m]), dev([0, n])
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 9.0)
+    try:
+        R.set_sm_budget(2)
+        monkeypatch.setenv("REAXMOE_WAIT_TIMEOUT_NS", "5000000")
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        _, lse = R.prompt_attention(q, k, v, c, ck, out=out, status=status, return_lse=True)
+        end.record()
+        torch.cuda.synchronize()
+    finally:
+        R.set_sm_budget(0)
+    assert int(status) == 0
+    assert start.elapsed_time(end) > 50          # ms: ten times the limit
+    assert torch.isnan(out[-1].float()).all()
+    rows = [0, 63, 126]
+    for r in rows:
+        ref = reference(q[r:r + 1], k[:n - m + r + 1], v[:n - m + r + 1], [0, 1], [0, n - m + r + 1], d ** -0.5)
+        check(out[r:r + 1], ref, lse[r:r + 1])
