@@ -205,6 +205,7 @@ class DecisionModel:
         self.max_positions = 0
         self._rope_cache = {}
         self.moe_stream = torch.cuda.Stream(self.dev)
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.dev)   # of this library's attention
         self.calibrated = False
         self.set_input_amax([8.0] * c.layers)
 
@@ -233,9 +234,24 @@ class DecisionModel:
             self.forward(token_ids, cu_seqlens, torch.zeros(1, dtype=torch.long, device=self.dev))
         finally:
             self._record = None
+        self._raise_status(self.read_status())
         self.set_input_amax(seen)
         self.calibrated = True
         return seen
+
+    # ------------------------------------------------------------------------------------------ device status
+    def read_status(self, clear: bool = True) -> int:
+        """Synchronise and return the status word of this library's attention: 0, or the code of a bounded wait that ran out,
+        after which some of its outputs were not written. :meth:`forward` returns NaN from then on, until this clears it."""
+        code = int(self._status)
+        if clear and code:
+            self._status.zero_()
+        return code
+
+    @staticmethod
+    def _raise_status(code: int) -> None:
+        if code:
+            raise L.ReaxMoEError(code, "a bounded wait of the attention kernel ran out")
 
     # ------------------------------------------------------------------------------------------ pieces
     def _cos_sin(self, max_len: int) -> None:
@@ -265,7 +281,7 @@ class DecisionModel:
         if prefix is not None or keep is not None or self.attention == "native":
             # the last query row of each prompt alone where `last` says so: the mask is aligned to the end of the keys
             cu_q = cu if last is None else torch.arange(last.numel() + 1, dtype=torch.int32, device=self.dev)
-            kw = dict(scale=1.0, window=c.window if c.sliding(layer) else None)
+            kw = dict(scale=1.0, window=c.window if c.sliding(layer) else None, status=self._status)
             qq = q if last is None else q[last]
             if prefix is None:
                 o = prompt_attention(qq, k, v, cu_q, cu, **kw)
@@ -336,7 +352,8 @@ class DecisionModel:
     @torch.no_grad()
     def prefill_prefix(self, token_ids: torch.Tensor) -> PrefixState:
         """Runs a prefix [length] that prompts will continue and keeps every layer's keys and values for
-        :meth:`forward` (``prefix``). Its own attention is this library's, whatever ``attention`` says."""
+        :meth:`forward` (``prefix``). Its own attention is this library's, whatever ``attention`` says. Waits for the result,
+        and raises ReaxMoEError if a bounded wait of the kernels ran out."""
         n = token_ids.numel()
         if n < 1:
             raise ValueError("a prefix has at least one token")
@@ -346,6 +363,7 @@ class DecisionModel:
         cu = torch.tensor([0, n], dtype=torch.int32, device=self.dev)
         state = PrefixState(n, [], [])
         state.last = self._layers(x, pos, cu, n, torch.tensor([n - 1], device=self.dev), keep=state)
+        self._raise_status(self.read_status())         # keys and values that are not whole are not kept
         return state
 
     @torch.no_grad()
@@ -353,12 +371,16 @@ class DecisionModel:
                 temperature: float = 1.0, prefix: PrefixState | None = None) -> torch.Tensor:
         """token_ids [N] (packed prompts), cu_seqlens [B + 1] int32 (device), option_ids [n_opt]. Returns the
         option probabilities [B, n_opt] float64 at each prompt's last position. ``prefix``: the prompts continue this one
-        (:meth:`prefill_prefix`), and token_ids holds only what follows it; a prompt of no tokens is the prefix itself."""
+        (:meth:`prefill_prefix`), and token_ids holds only what follows it; a prompt of no tokens is the prefix itself.
+        Probabilities are NaN, and the next call raises ReaxMoEError, if a bounded wait of this library's attention ran out."""
         c = self.cfg
         cu = cu_seqlens.to(device=self.dev, dtype=torch.int32)
         n = token_ids.numel()
         lens = cu[1:] - cu[:-1]
-        max_len, min_len = torch.stack([lens.max(), lens.min()]).tolist()
+        max_len, min_len, code = torch.stack([lens.max(), lens.min(), self._status[0]]).tolist()
+        if code:
+            self._status.zero_()
+            self._raise_status(code)
         start = 0 if prefix is None else prefix.length
         if prefix is not None and len(prefix.keys) != c.layers:
             raise ValueError(f"the prefix has {len(prefix.keys)} layers, the model {c.layers}")
@@ -388,6 +410,8 @@ class DecisionModel:
         if c.final_softcap:
             logits = torch.tanh(logits / c.final_softcap) * c.final_softcap
         opt = logits[:, option_ids.to(self.dev).long()].double() / temperature
+        if self.attention == "native" or prefix is not None:
+            opt = opt.masked_fill(self._status != 0, float("nan"))
         return torch.softmax(opt, dim=-1)
 
 

@@ -57,3 +57,37 @@ def test_a_prefix_without_its_last_row_is_refused_for_such_prompts():
     with pytest.raises(ValueError):
         model.forward(*packed([tails[0], torch.zeros(0, dtype=torch.long)]), opts, prefix=bare)
     model.forward(*packed(tails), opts, prefix=bare)
+
+
+def test_a_wait_that_ran_out_is_not_passed_over(monkeypatch):
+    """Every attention call is given the model's status word; a code in it makes the results NaN and the next call raise, keeps a
+    prefix from being handed out, and is gone then. (The code is written by the host here.)"""
+    from reax_engine_b200 import _lib as L
+    from reax_engine_b200 import decision
+    model, head, tails, state, opts = prefixed()
+    ids, cu = packed(tails)
+    good, good_prefix = model.forward(ids, cu, opts), model.forward(ids, cu, opts, prefix=state)
+    calls = []
+    for name in ("prompt_attention", "shared_prefix_attention"):
+        def failing(*a, real=getattr(decision, name), status, **kw):
+            calls.append(status)
+            if len(calls) % 2:                                 # of the two layers the first
+                status.fill_(L.ERR_DEVICE_TIMEOUT)
+            return real(*a, status=status, **kw)
+        monkeypatch.setattr(decision, name, failing)
+    for prefix in (None, state):
+        assert torch.isnan(model.forward(ids, cu, opts, prefix=prefix)).all()
+        with pytest.raises(L.ReaxMoEError) as e:
+            model.forward(ids, cu, opts)
+        assert e.value.code == L.ERR_DEVICE_TIMEOUT and len(calls) % 2 == 0
+    with pytest.raises(L.ReaxMoEError):
+        model.prefill_prefix(head.cuda())
+    assert torch.isnan(model.forward(ids, cu, opts)).all() and model.read_status() == L.ERR_DEVICE_TIMEOUT
+    before = list(model.input_amax)
+    with pytest.raises(L.ReaxMoEError):
+        model.calibrate(ids, cu)
+    assert model.input_amax == before
+    monkeypatch.undo()
+    assert model.read_status() == 0
+    assert torch.equal(model.forward(ids, cu, opts), good)
+    assert torch.equal(model.forward(ids, cu, opts, prefix=state), good_prefix)
