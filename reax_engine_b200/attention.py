@@ -25,11 +25,35 @@ _DTYPES = {torch.bfloat16: L.BF16, torch.float16: L.FP16}
 _checked: dict = {}
 _unused: dict = {}        # device -> the workspace of calls that use none
 _CHECKED_MAX = 4096
+_status: dict = {}        # device -> the status word of calls that are given none
 _UNUSED = 16             # a workspace of this size is never touched (reaxmoe_attention_workspace_size)
 
 
 def forget_checked() -> None:
     _checked.clear()
+
+
+def attention_status(device: torch.device | str | int | None = None, clear: bool = True) -> int:
+    """Synchronise the current stream of ``device`` (default: the current one) and return the status word of the attention calls
+    there that were given none: 0, or the code of a bounded wait that ran out in one of them, whose output is then not whole."""
+    device = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError("attention runs on CUDA devices")
+    word = _status.get(device if device.index is not None else torch.device("cuda", torch.cuda.current_device()))
+    if word is None:
+        return 0
+    code = int(word)
+    if clear and code:
+        word.zero_()
+    return code
+
+
+def _default_status(device: torch.device) -> torch.Tensor | None:
+    """The device's status word: none before the first call of a process that is not being captured (which could not zero it)."""
+    word = _status.get(device)
+    if word is None and not torch.cuda.is_current_stream_capturing():
+        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return word
 
 
 def _readable(t: torch.Tensor) -> bool:
@@ -122,7 +146,11 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         dst = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=q.dtype, device=device)
     else:
         dst = _output(out, q, (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v))
-    if status is not None and (status.dtype != torch.int32 or status.device != device or status.numel() < 1):
+    if status is None:
+        status = _status.get(device)
+        if status is None:
+            status = _default_status(device)
+    elif status.dtype != torch.int32 or status.device != device or status.numel() < 1:
         raise ValueError("status must be an int32 tensor on the device of q")
     if scale is not None:
         scale = float(scale)
@@ -198,7 +226,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``return_lse`` the natural logarithm of the softmax's sum [tokens, heads] fp32 too.
 
     ``workspace``: a uint8 buffer of at least ``reaxmoe_attention_workspace_size`` bytes, used by one call at a time (default:
-    one from torch's allocator for this call). ``status``: an optional int32 device tensor that receives a device-timeout code.
+    one from torch's allocator for this call). ``status``: an int32 device tensor that receives a device-timeout code if a bounded
+    wait of the kernel runs out, in which case rows of the output are missing (default: a word per device,
+    :func:`attention_status`).
     """
     return _attention(q, k, v, None, None, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out, workspace, status)
 

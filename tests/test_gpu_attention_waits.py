@@ -61,3 +61,18 @@ def test_rows_done_key_by_key_do_not_run_out_the_waits_for_them(monkeypatch, d):
     for r in rows:
         ref = reference(q[r:r + 1], k[:n - m + r + 1], v[:n - m + r + 1], [0, 1], [0, n - m + r + 1], d ** -0.5)
         check(out[r:r + 1], ref, lse[r:r + 1])
+
+
+def test_a_call_without_a_status_word_is_reported(monkeypatch):
+    import reax_engine_b200 as R
+    from reax_engine_b200 import _lib as L
+    c = dev([0, 3000])
+    q, k, v, _, _ = tensors(3000, 3000, 8, 4, 128, "bf16", 1)
+    want = R.prompt_attention(q, k, v, c)
+    assert R.attention_status() == 0
+    monkeypatch.setenv("REAXMOE_WAIT_TIMEOUT_NS", "0")
+    R.prompt_attention(q, k, v, c)
+    monkeypatch.delenv("REAXMOE_WAIT_TIMEOUT_NS")
+    assert R.attention_status("cuda:0", clear=False) == L.ERR_DEVICE_TIMEOUT
+    assert R.attention_status(0) == L.ERR_DEVICE_TIMEOUT and R.attention_status(torch.device("cuda")) == 0
+    assert torch.equal(R.prompt_attention(q, k, v, c), want) and R.attention_status() == 0
