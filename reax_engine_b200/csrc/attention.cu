@@ -559,12 +559,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       return true;
     };
     // The halves of a row exchange a value (maximum, sum) through one word each, whose lowest bit says which use of the word it
-    // is: a word is used every other time, and written again only after the other side has gone on to the next one. Both
-    // sides go on with the same two words, without that bit.
-    auto post = [&](float v) {
-      sts_volatile(x_mine + (uint32_t)((x_n & 1) * 2 * ROWS * 4), (__float_as_uint(v) & ~1u) | (uint32_t)((x_n >> 1) & 1));
+    // is: a word is used every other time, and written again only after the other side has gone on to the next one.
+    // A maximum gives up its lowest bit for it, on both sides: it only says what the weights are relative to, so nothing is lost.
+    // A sum keeps all its bits: it has no sign, whose place the shift frees.
+    auto post = [&](uint32_t bits) {
+      sts_volatile(x_mine + (uint32_t)((x_n & 1) * 2 * ROWS * 4), bits | (uint32_t)((x_n >> 1) & 1));
     };
-    auto receive = [&](float& other) {
+    auto receive = [&](uint32_t& other) {
       const uint32_t at = x_other + (uint32_t)((x_n & 1) * 2 * ROWS * 4), tag = (uint32_t)((x_n >> 1) & 1);
       ++x_n;
       uint32_t v = lds_volatile(at);
@@ -585,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
         }
         v = lds_volatile(at);
       }
-      other = __uint_as_float(v & ~1u);
+      other = v & ~1u;
       return true;
     };
     auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & ~1u); };   // as the other side gets it
@@ -699,13 +700,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
           mx[1] = max3_nan(mx[1], __uint_as_float(x1[x]), __uint_as_float(x1[x + 1]));
         }
         mine = cut(max_nan(mx[0], mx[1]));
-        post(mine);
+        post(__float_as_uint(mine));
       };
       // the softmax of one tile whose scores are in registers and whose half maxima are posted
       auto weigh = [&](const Tile& t, uint32_t (&x0)[32], uint32_t (&x1)[32]) {
-        float top;
-        if (!receive(top)) return false;
-        top = max_nan(top, mine) * c;
+        uint32_t other;
+        if (!receive(other)) return false;
+        const float top = max_nan(__uint_as_float(other), mine) * c;
         if (!(top < INFINITY)) l = NAN;          // a score that is NaN or infinite: so are the row's weights
         const bool grow = top - m > THR;         // from -inf on the first key
         const bool rescale = grow && m != -INFINITY;
@@ -775,10 +776,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       if (!ok) break;
       // the sums, for the output warps
       if (any_live) {
-        float other;
-        post(l);
+        uint32_t other;
+        post(__float_as_uint(l) << 1);
         if (!(ok = receive(other))) break;
-        l = cut(l) + other;
+        l += __uint_as_float(other >> 1);
       }
       if (half == 0) {
         if (i > 0 && !(ok = wait(l_empty, (uint32_t)(i - 1)))) break;

@@ -23,3 +23,18 @@ def test_lengths_that_do_not_rise_from_zero(d, prefix, keys):
         call(bad, ck)
         call(cq, [keys - 1, -5, 2 ** 31 - 1, 3] + [-2 ** 31, 7] * 5)
     check(call(cq, ck)[9:], [x[9:] for x in ref])
+
+
+def test_row_sums_keep_all_their_bits():
+    """Weights 1 and 2^-23 (scale ln 2, whose product with log2(e) is 1 in fp32) of values 1 and 12288: the sum of the products is
+    1 + 3 2^-11, half-way between two fp16 values, and the sum of the weights, 1 + 2^-23, decides that the lower one is nearer."""
+    import math
+    import reax_engine_b200 as R
+    q, k, v = (torch.zeros(2, 1, 64, dtype=torch.float16, device="cuda") for _ in range(3))
+    q[..., 0] = 1
+    k[1, 0, 0] = -23
+    v[0], v[1] = 1, 12288
+    for first in (0, 1):                     # either key first: the halves of the columns add up in another order
+        kk, vv = (k, v) if first == 0 else (k.flip(0), v.flip(0))
+        o = R.prompt_attention(q, kk, vv, dev([0, 2]), causal=False, scale=math.log(2))
+        assert (o == 1 + 2.0 ** -10).all()
