@@ -83,7 +83,7 @@ def _output(out: torch.Tensor, q: torch.Tensor, inputs) -> torch.Tensor:
     """What the kernels write for the caller's `out`: itself, or a copy where its rows cannot be addressed."""
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have the shape, dtype and device of q")
-    if any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in inputs):
+    if out.numel() and any(out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in inputs):   # (none: 0)
         raise ValueError("out must not share its storage with an input")
     if out.ndim != 3:
         raise ValueError("q must be [tokens, heads, head_dim]")

@@ -38,3 +38,11 @@ def test_row_sums_keep_all_their_bits():
         kk, vv = (k, v) if first == 0 else (k.flip(0), v.flip(0))
         o = R.prompt_attention(q, kk, vv, dev([0, 2]), causal=False, scale=math.log(2))
         assert (o == 1 + 2.0 ** -10).all()
+
+
+def test_an_empty_batch_into_an_output():
+    import reax_engine_b200 as R
+    q, k, v, pk, pv = tensors(0, 0, 4, 2, 64, "bf16", 1, prefix=5)
+    out = torch.empty_like(q)
+    assert R.prompt_attention(q, k, v, dev([0, 0]), out=out) is out
+    assert R.shared_prefix_attention(q, k, v, pk, pv, dev([0]), out=out) is out
