@@ -189,7 +189,7 @@ typedef struct reaxmoe_attention_args {
   const void* prefix_v;
   const int32_t* cu_q;        /* [seqs + 1], non-decreasing from 0 (device) */
   const int32_t* cu_k;        /* [seqs + 1] */
-  void* out;                  /* [q_tokens, q_heads, head_dim] in the type of q; overlaps no input */
+  void* out;                  /* [q_tokens, q_heads, head_dim] in the type of q; overlaps no input, nor its own rows one another */
   float* lse;                 /* [q_tokens, q_heads] or NULL */
   int32_t* status;            /* device word or NULL: receives REAXMOE_ERR_DEVICE_TIMEOUT if a bounded wait expires */
   /* strides in elements, between tokens and between heads (the last dimension is contiguous); multiples of 8 */

@@ -479,6 +479,16 @@ static bool bad_strides(int64_t token, int64_t head, int heads, int64_t tokens, 
   return tokens > 1 && token < d;
 }
 
+// whether two rows of d elements at t * token + h * head (t < tokens, h < heads) share an element; strides as above
+static bool rows_overlap(int64_t token, int64_t head, int heads, int64_t tokens, int d) {
+  if (heads < 2 || tokens < 2 || (token - d) / (heads - 1) >= head || (head - d) / (tokens - 1) >= token) return false;
+  for (int64_t h = 1; h < heads; ++h) {          // h heads apart: the two tokens whose distance comes nearest
+    const int64_t t = h * head / token, rest = h * head - t * token;
+    if ((t < tokens && rest < d) || (t + 1 < tokens && token - rest < d)) return true;
+  }
+  return false;
+}
+
 size_t reaxmoe_attention_workspace_size(const reaxmoe_attention_args* args) {
   if (check_attention_sizes(args)) return 0;
   return attention_workspace(*args, num_sms());
@@ -502,6 +512,8 @@ int reaxmoe_attention(const reaxmoe_attention_args* args, void* workspace, size_
       (a.prefix > 0 && (bad_strides(a.prefix_k_stride, a.prefix_k_head_stride, a.kv_heads, a.prefix, d) ||
                         bad_strides(a.prefix_v_stride, a.prefix_v_head_stride, a.kv_heads, a.prefix, d))))
     return fail(REAXMOE_ERR_MISALIGNED, "attention: strides must be multiples of 8 elements and rows must not overlap");
+  if (rows_overlap(a.out_stride, a.out_head_stride, a.q_heads, a.q_tokens, d))
+    return fail(REAXMOE_ERR_MISALIGNED, "attention: rows of out must not overlap");
   AttentionLaunch l;
   memset(&l, 0, sizeof(l));
   l.a = a;

@@ -17,3 +17,18 @@ def test_an_empty_output_shares_nothing():
     t = torch.empty(3, 4, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         A._output(t[1:], t[:2], (t,))
+
+
+def test_rows_of_the_output_must_not_overlap():
+    """Token and head strides that are each wide enough, together (100 tokens, 16 heads of 64)."""
+    bad = [(64, 64), (128, 64), (512, 64), (1024 - 8, 64), (64, 128), (64, 6400 - 8), (128, 192), (64 * 7, 64 * 3)]
+    good = [(1024, 64), (1032, 64), (2048, 128), (64, 6400), (72, 7200), (64, 1 << 20), (1 << 20, 64), (64 * 33, 64 * 2),
+            (64 * 17, 64 * 2 * 17 + 64)]
+    rows = lambda t, h: [i * t + j * h for i in range(100) for j in range(16)]  # noqa: E731
+    for t, h in bad + good:
+        at = sorted(rows(t, h))
+        overlap = any(b - a < 64 for a, b in zip(at, at[1:]))
+        assert call(out_stride=t, out_head_stride=h) == (L.ERR_MISALIGNED if overlap else L.ERR_WORKSPACE), (t, h)
+    assert any(b - a < 64 for t, h in bad for a, b in zip(sorted(rows(t, h)), sorted(rows(t, h))[1:]))
+    # inputs may (a broadcast or sliding view reads the same elements twice)
+    assert call(k_stride=64) == L.ERR_WORKSPACE
