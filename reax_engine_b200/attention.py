@@ -108,14 +108,14 @@ def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError("scale must be positive and finite")
-    if window is not None and (not causal or int(window) < 1):
+    if window is not None and (not causal or window < 1):
         raise ValueError("window must be at least 1, with causal=True")
     if seqs_k != seqs:
         raise ValueError("cu_seqlens and cu_seqlens_k must have the same length")
     strides = [x for t in (q, k, v, prefix_k, prefix_v, dst) for x in ((0, 0) if t is None else t.stride()[:2])]
     args = L.AttentionArgs(*([None] * 10), *strides, q.shape[0], k.shape[0], 0 if prefix_k is None else prefix_k.shape[0],
-                           seqs - 1, q.shape[1], k.shape[1], d, _DTYPES[q.dtype], int(bool(causal)),
-                           0 if window is None else min(int(window), 0x7FFFFFFF), scale)
+                           seqs - 1, q.shape[1], k.shape[1], d, _DTYPES[q.dtype], int(causal),
+                           0 if window is None else min(window, 0x7FFFFFFF), scale)
     need = L.lib().reaxmoe_attention_workspace_size(ctypes.byref(args))
     if need == 0:
         raise L.ReaxMoEError(L.ERR_BAD_SHAPE, L.last_error())
@@ -154,6 +154,9 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         raise ValueError("status must be an int32 tensor on the device of q")
     if scale is not None:
         scale = float(scale)
+    if window is not None:
+        window = int(window)
+    causal = bool(causal)           # values, not what held them: they are part of the key below
     key = (device, shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
            dst.stride(), cu_q.shape, cu_k.shape, scale, causal, window)
     aligned = _aligned(q) and _aligned(k) and _aligned(v)

@@ -46,3 +46,20 @@ def test_an_empty_batch_into_an_output():
     out = torch.empty_like(q)
     assert R.prompt_attention(q, k, v, dev([0, 0]), out=out) is out
     assert R.shared_prefix_attention(q, k, v, pk, pv, dev([0]), out=out) is out
+
+
+def test_options_that_are_written_in_place():
+    """Options given as tensors count with what they hold at the call."""
+    import reax_engine_b200 as R
+    q, k, v, _, _ = tensors(40, 40, 4, 2, 64, "bf16", 5)
+    c = dev([0, 40])
+    window, causal, scale = torch.tensor(3), torch.tensor(True), torch.tensor(0.125)
+    for w, cs, s in ((3, True, 0.125), (20, True, 0.125), (20, True, 0.5), (3, True, 0.125)):
+        window.fill_(w), causal.fill_(cs), scale.fill_(s)
+        got = R.prompt_attention(q, k, v, c, window=window, causal=causal, scale=scale)
+        assert torch.equal(got, R.prompt_attention(q, k, v, c, window=w, causal=cs, scale=s))
+        check(got, reference(q, k, v, [0, 40], [0, 40], s, window=w))
+    causal.fill_(False)
+    assert torch.equal(R.prompt_attention(q, k, v, c, causal=causal), R.prompt_attention(q, k, v, c, causal=False))
+    with pytest.raises(ValueError):
+        R.prompt_attention(q, k, v, c, causal=causal, window=window)
