@@ -14,6 +14,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .moe import _require_cuda
@@ -122,6 +123,14 @@ def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window
     return bytes(args), need
 
 
+def _no_gradients(ts) -> None:
+    for t in ts:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError("this attention has no forward-mode derivative: unpack its inputs")
+
+
 def _aligned(t: torch.Tensor) -> bool:
     return t.data_ptr() % 16 == 0
 
@@ -134,9 +143,7 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         with torch.cuda.device(device):
             return _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out,
                               workspace, status)
-    if (q.requires_grad or k.requires_grad or v.requires_grad or (prefix_k is not None and (
-            prefix_k.requires_grad or prefix_v.requires_grad))) and torch.is_grad_enabled():
-        raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
+    _no_gradients((q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v))
     cu_q = _lengths(cu_seqlens, "cu_seqlens", device)
     cu_k = cu_q if cu_seqlens_k is None else _lengths(cu_seqlens_k, "cu_seqlens_k", device)
     shape = q.shape

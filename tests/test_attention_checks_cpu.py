@@ -32,3 +32,22 @@ def test_rows_of_the_output_must_not_overlap():
     assert any(b - a < 64 for t, h in bad for a, b in zip(sorted(rows(t, h)), sorted(rows(t, h))[1:]))
     # inputs may (a broadcast or sliding view reads the same elements twice)
     assert call(k_stride=64) == L.ERR_WORKSPACE
+
+
+def test_inputs_that_carry_derivatives():
+    from torch.autograd import forward_ad
+    x, y = torch.ones(2, 1, 64), torch.ones(2, 1, 64)
+    A._no_gradients((x, y))
+    with pytest.raises(ValueError):
+        A._no_gradients((x, y.clone().requires_grad_()))
+    with torch.no_grad():
+        A._no_gradients((x, y.clone().requires_grad_()))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for ts in ((dual, y), (y, dual), (y, dual[:1])):
+            with pytest.raises(ValueError):
+                A._no_gradients(ts)
+            with torch.no_grad(), pytest.raises(ValueError):
+                A._no_gradients(ts)
+        A._no_gradients((y, forward_ad.unpack_dual(dual).primal))
+    A._no_gradients((x, y))

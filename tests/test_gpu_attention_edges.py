@@ -63,3 +63,17 @@ def test_options_that_are_written_in_place():
     assert torch.equal(R.prompt_attention(q, k, v, c, causal=causal), R.prompt_attention(q, k, v, c, causal=False))
     with pytest.raises(ValueError):
         R.prompt_attention(q, k, v, c, causal=causal, window=window)
+
+
+def test_tangents_are_refused():
+    import reax_engine_b200 as R
+    from torch.autograd import forward_ad
+    q, k, v, pk, pv = tensors(8, 8, 4, 2, 64, "bf16", 2, prefix=4)
+    c = dev([0, 8])
+    R.shared_prefix_attention(q, k, v, pk, pv, c)            # (checked calls are remembered)
+    with forward_ad.dual_level():
+        for i in range(5):
+            ts = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate((q, k, v, pk, pv))]
+            with pytest.raises(ValueError):
+                R.shared_prefix_attention(*ts, c)
+        R.shared_prefix_attention(q, k, v, pk, pv, c)
