@@ -136,6 +136,8 @@ def _aligned(t: torch.Tensor) -> bool:
 
 
 def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out, workspace, status):
+    if (prefix_k is None) != (prefix_v is None):
+        raise ValueError("prefix_k and prefix_v go together")
     device = q.device
     if device.type != "cuda":
         _require_cuda(q)

@@ -51,3 +51,11 @@ def test_inputs_that_carry_derivatives():
                 A._no_gradients(ts)
         A._no_gradients((y, forward_ad.unpack_dual(dual).primal))
     A._no_gradients((x, y))
+
+
+def test_half_a_prefix():
+    import reax_engine_b200 as R
+    t, c = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+    for pk, pv in ((t, None), (None, t)):
+        with pytest.raises(ValueError, match="go together"):
+            R.shared_prefix_attention(t, t, t, pk, pv, c)
