@@ -200,7 +200,7 @@ typedef struct reaxmoe_attention_args {
   int32_t dtype;              /* REAXMOE_BF16 or REAXMOE_FP16 */
   int32_t causal;             /* 0 or 1 */
   int32_t window;             /* 0: none; else >= 1, with causal */
-  float scale;                /* > 0 */
+  float scale;                /* > 0, at most 2.3e38 */
 } reaxmoe_attention_args;
 
 /* Bytes of workspace reaxmoe_attention needs for these sizes (0 on bad sizes; 16: none is touched, any 16 bytes will do). It

@@ -466,8 +466,8 @@ static int check_attention_sizes(const reaxmoe_attention_args* a) {
     return fail(REAXMOE_ERR_UNSUPPORTED, "attention: dtype=%d (bf16 or fp16)", a->dtype);
   if ((a->causal != 0 && a->causal != 1) || a->window < 0 || (a->window > 0 && !a->causal))
     return fail(REAXMOE_ERR_BAD_SHAPE, "attention: causal=%d window=%d (a window needs causal)", a->causal, a->window);
-  if (!(a->scale > 0.0f) || a->scale > 3.0e38f)
-    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: scale must be positive and finite");
+  if (!(a->scale > 0.0f) || a->scale > 2.3e38f)    // the kernels use scale log2(e)
+    return fail(REAXMOE_ERR_BAD_SHAPE, "attention: scale must be positive and at most 2.3e38");
   return 0;
 }
 

@@ -6,7 +6,7 @@ import torch
 
 from reax_engine_b200 import _lib as L
 from reax_engine_b200 import attention as A
-from test_attention_cpu import call
+from test_attention_cpu import BASE, call
 
 
 def test_an_empty_output_shares_nothing():
@@ -59,3 +59,11 @@ def test_half_a_prefix():
     for pk, pv in ((t, None), (None, t)):
         with pytest.raises(ValueError, match="go together"):
             R.shared_prefix_attention(t, t, t, pk, pv, c)
+
+
+def test_a_scale_whose_product_with_log2_e_is_infinite():
+    """2.4e38 log2(e) is past fp32's range: every weight would be NaN."""
+    for s in (2.4e38, 2.9e38, 3.4e38):
+        a = L.AttentionArgs(**{**BASE, "scale": s})
+        assert L.lib().reaxmoe_attention_workspace_size(ctypes.byref(a)) == 0 and call(scale=s) == L.ERR_BAD_SHAPE
+    assert call(scale=2.2e38) == L.ERR_WORKSPACE
