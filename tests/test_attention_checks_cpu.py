@@ -67,3 +67,19 @@ def test_a_scale_whose_product_with_log2_e_is_infinite():
         a = L.AttentionArgs(**{**BASE, "scale": s})
         assert L.lib().reaxmoe_attention_workspace_size(ctypes.byref(a)) == 0 and call(scale=s) == L.ERR_BAD_SHAPE
     assert call(scale=2.2e38) == L.ERR_WORKSPACE
+
+
+def test_the_plan_that_other_tests_go_by():
+    import random
+    from attention_plan import plan
+    rng = random.Random(3)
+    for _ in range(3000):
+        kv, d = rng.choice([1, 2, 4, 8, 16]), rng.choice([64, 128, 256])
+        hq = kv * rng.choice([1, 2, 4, 5, 8, 16, 17])
+        seqs = rng.choice([1, 2, 7, 64, 300])
+        nq = rng.choice([1, seqs, seqs + 1, seqs * 40])
+        nk = rng.choice([nq, 16 * seqs - 1, 16 * seqs, 4095, 4096, 32767, 32768, 200000])
+        prefix = rng.choice([0, 0, 1, 512, 513, 20000])
+        a = L.AttentionArgs(**{**BASE, "q_tokens": nq, "k_tokens": nk, "seqs": seqs, "q_heads": hq, "kv_heads": kv, "head_dim": d,
+                               "prefix": prefix})
+        assert L.lib().reaxmoe_attention_workspace_size(ctypes.byref(a)) == plan(nq, nk, seqs, hq, kv, d, prefix).workspace
