@@ -7,6 +7,12 @@
 // b that overlap have the number u = c + b (a staircase: there are at most chunks + sequences of them, and b is found from u by
 // bisection), under which the unit's partial maximum, sum and output stand for join_kernel. Units do not wait for one another.
 //
+// A sequence may have more rows than a unit's 16 all the same (a batch with unused slots, a chunk of a prompt in one of the others).
+// Its units then do not share out its keys but its rows: the i-th takes rows 16 i .. 16 i + 15 and all keys that these see.
+// Rows behind the last unit's (only where there are far fewer keys than rows) are done one by one. 4 sequences of 60 tokens and
+// 20000 keys each in 256 slots: 0.94 ms at D = 128 (32 / 8 heads), 1.87 at D = 256 (16 / 8); one by one all rows took 14.4 and
+// 18.0, and without the unused slots, in tiles, it is 0.28 and 0.24.
+//
 // Per 16 keys, rows m = 16 (unused ones are zero): S = Q K^T and O += P V by mma.m16n8k16, Q in registers, K and V in a ring of
 // 16-row slots that 16-byte asynchronous copies fill (rows are D * 2 bytes, 16 bytes of padding keep ldmatrix free of
 // conflicts). One bulk copy per row instead took 20 to 30 clocks of the copy engine each: 3.3 TB/s at D = 128.
@@ -70,7 +76,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // A unit of work of one warp: keys [from, to) of one sequence for one KV head.
 struct Unit {
   int u, head;
-  int q0, rows;              // the sequence's first query token, its query rows (of this head); rows == 0: nothing to do
+  int q0, row0, rows;        // the sequence's first query token; the unit's rows of it (for this head); rows == 0: nothing to do
   int from, to;
   int lo0, hi0, lo1, hi1;    // keys that this thread's two rows see
 };
@@ -81,7 +87,7 @@ __device__ __forceinline__ Unit find_unit(const FewParams& p, int task, int ntok
   Unit w;
   w.u = task / p.a.kv_heads;
   w.head = task - w.u * p.a.kv_heads;
-  w.rows = w.from = w.to = 0;
+  w.row0 = w.rows = w.from = w.to = 0;
   // the last b whose first unit, cu_k[b] / chunk + b, is not beyond u
   int b = 0, len = p.a.seqs;
 #pragma unroll 1
@@ -99,12 +105,20 @@ __device__ __forceinline__ Unit find_unit(const FewParams& p, int task, int ntok
   w.q0 = max(qa, 0);
   const int q1 = min(sq.q_end, ntok);
   if (sq.ks >= ke || c < sq.ks / p.chunk || c > (ke - 1) / p.chunk) return w;            // the staircase has none here
-  if (w.q0 >= q1 || q1 - w.q0 > FEW_ROWS || (q1 - w.q0) * p.group > FEW_ROWS) return w;   // none, or join_kernel's to do
-  w.rows = (q1 - w.q0) * p.group;
-  const RowKeys k0 = row_keys_in(p.a, sq, w.q0 + min(lane >> 2, w.rows - 1) / p.group);
-  const RowKeys k1 = row_keys_in(p.a, sq, w.q0 + min((lane >> 2) + 8, w.rows - 1) / p.group);
-  w.from = max(c * p.chunk, row_keys_in(p.a, sq, w.q0).k_lo);
-  w.to = (int)min((int64_t)(c + 1) * p.chunk, (int64_t)row_keys_in(p.a, sq, q1 - 1).k_hi);
+  if (w.q0 >= q1) return w;
+  const int total = (q1 - w.q0) * p.group;
+  const bool by_rows = total > FEW_ROWS;
+  if (by_rows) w.row0 = (c - sq.ks / p.chunk) * FEW_ROWS;
+  if (w.row0 >= total) return w;
+  w.rows = min(total - w.row0, FEW_ROWS);
+  auto token = [&](int r) { return w.q0 + (w.row0 + min(r, w.rows - 1)) / p.group; };      // of the unit's row r
+  const RowKeys k0 = row_keys_in(p.a, sq, token(lane >> 2)), k1 = row_keys_in(p.a, sq, token((lane >> 2) + 8));
+  w.from = row_keys_in(p.a, sq, token(0)).k_lo;
+  w.to = row_keys_in(p.a, sq, token(FEW_ROWS)).k_hi;
+  if (!by_rows) {
+    w.from = max(c * p.chunk, w.from);
+    w.to = (int)min((int64_t)(c + 1) * p.chunk, (int64_t)w.to);
+  }
   w.lo0 = k0.k_lo;
   w.hi0 = min(k0.k_hi, w.to);
   w.lo1 = k1.k_lo;
@@ -130,7 +144,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewLayout<D>::BLOCKS) few_kern
   if (task < tasks) w = find_unit(p, task, ntok);
 #pragma unroll 1
   while (task < tasks) {
-    const int rows = w.rows, q0 = w.q0, head = w.head, from = w.from, to = w.to;
+    const int rows = w.rows, q0 = w.q0, row0 = w.row0, head = w.head, from = w.from, to = w.to;
     const int lo0 = w.lo0, hi0 = w.hi0, lo1 = w.lo1, hi1 = w.hi1;
     const int64_t at_row = ((int64_t)head * p.units + w.u) * FEW_ROWS;
     task += FEW_WARPS * gridDim.x;
@@ -169,8 +183,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewLayout<D>::BLOCKS) few_kern
     uint32_t q[D / 16][4];
     {
       const uint16_t* qb = static_cast<const uint16_t*>(p.a.q) + (int64_t)head * p.group * p.a.q_head_stride + (lane & 3) * 2;
-      const uint16_t* qa = qb + (int64_t)(q0 + r0 / p.group) * p.a.q_stride + (int64_t)(r0 % p.group) * p.a.q_head_stride;
-      const uint16_t* qc = qb + (int64_t)(q0 + r1 / p.group) * p.a.q_stride + (int64_t)(r1 % p.group) * p.a.q_head_stride;
+      const int qr0 = row0 + r0, qr1 = row0 + r1;
+      const uint16_t* qa = qb + (int64_t)(q0 + qr0 / p.group) * p.a.q_stride + (int64_t)(qr0 % p.group) * p.a.q_head_stride;
+      const uint16_t* qc = qb + (int64_t)(q0 + qr1 / p.group) * p.a.q_stride + (int64_t)(qr1 % p.group) * p.a.q_head_stride;
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
         q[x][0] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(qa + x * 16)) : 0u;
@@ -311,16 +326,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
   const Sequence sq = sequence_at(p.a, b);
   const int q0 = max(__ldg(p.a.cu_q + b), 0), q1 = min(sq.q_end, ntok);
   const int kvh = head / p.group, row = (tok - q0) * p.group + head - kvh * p.group;
-  // too many rows for few_kernel (or, where the lengths do not rise from 0, a row outside its sequence, which has no place there)
-  if (q1 - q0 > FEW_ROWS || (q1 - q0) * p.group > FEW_ROWS || tok < q0 || tok >= q1) {
+  const int ke = sq.ks + sq.all - (int)p.a.prefix;
+  const int first = sq.ks / p.chunk + b, units = sq.ks < ke ? (ke - 1) / p.chunk + b - first + 1 : 0;
+  const bool inside = tok >= q0 && tok < q1;         // (not where the lengths do not rise from 0)
+  const bool by_rows = inside && (q1 - q0) * p.group > FEW_ROWS;
+  if (!inside || (by_rows && units > 0 && row / FEW_ROWS >= units)) {
     if (warp == 0) row_by_warp<D, BF>(p.a, tok, head, true);
     return;
   }
-  const int ke = sq.ks + sq.all - (int)p.a.prefix;
-  const int first = sq.ks / p.chunk + b, own = sq.ks < ke ? (ke - 1) / p.chunk + b - first + 1 : 0;
+  const int own = by_rows ? min(units, 1) : units, unit = first + (by_rows ? row / FEW_ROWS : 0);
   const int n = own + p.prefix_parts;
   // partial result i of n: the units of the row's own keys, then the prefix's parts
-  const int64_t unit0 = ((int64_t)kvh * p.units + first) * FEW_ROWS + row;
+  const int64_t unit0 = ((int64_t)kvh * p.units + unit) * FEW_ROWS + row % FEW_ROWS;
   const int64_t part0 = (int64_t)kvh * p.prefix_rows + (int64_t)tok * p.group + head - kvh * p.group;
   const int64_t part_step = (int64_t)p.a.kv_heads * p.prefix_rows;
   auto ml = [&](int i) { return i < own ? p.ml[unit0 + (int64_t)i * FEW_ROWS] : p.prefix_ml[part0 + (i - own) * part_step]; };

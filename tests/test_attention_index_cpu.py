@@ -57,24 +57,45 @@ def test_generation_step_stays_inside(kind):
         units, ntok = -(-k_tokens // chunk) + seqs, min(cu_q[seqs], q_tokens)
         at = lambda b: sequence_at(cu_q, cu_k, b, prefix, k_tokens, q_tokens)  # noqa: E731
         keys = lambda s, t: row_keys_in(s, t, prefix, k_tokens, causal, window)  # noqa: E731
+        done = {}                                             # first row of a unit's 16 (by sequence), its keys: by unit
         for u in range(units):                                # find_unit
             b = sequence_by_warp(lambda i: min(max(cu_k[i], 0), k_tokens) // chunk + i <= u, seqs)
             s, c = at(b), u - b
             q0, q1, ke = max(cu_q[b], 0), min(s[2], ntok), s[0] + s[1] - prefix
-            if s[0] >= ke or not s[0] // chunk <= c <= (ke - 1) // chunk or q0 >= q1 or (q1 - q0) * group > ROWS:
+            if s[0] >= ke or not s[0] // chunk <= c <= (ke - 1) // chunk or q0 >= q1:
                 continue
-            assert q1 <= q_tokens
-            first, last = max(c * chunk, keys(s, q0)[0]), min((c + 1) * chunk, keys(s, q1 - 1)[1])
+            total = (q1 - q0) * group
+            row0 = (c - s[0] // chunk) * ROWS if total > ROWS else 0
+            if row0 >= total:
+                continue
+            rows = min(total - row0, ROWS)
+            token = lambda r: q0 + (row0 + min(r, rows - 1)) // group  # noqa: E731
+            assert q0 <= token(0) <= token(ROWS) < q1 <= q_tokens
+            first, last = keys(s, token(0))[0], keys(s, token(ROWS))[1]
+            if total <= ROWS:
+                first, last = max(c * chunk, first), min((c + 1) * chunk, last)
             assert first >= last or 0 <= first < last <= k_tokens
+            done[u] = b, row0, rows, first, last
         for tok in range(ntok):                               # join_kernel
             b = sequence_by_warp(lambda i: cu_q[i] <= tok, seqs)
             s = at(b)
-            keys(s, tok)
+            k_lo, k_hi = keys(s, tok)
             q0, q1, ke = max(cu_q[b], 0), min(s[2], ntok), s[0] + s[1] - prefix
-            if (q1 - q0) * group > ROWS or tok < q0 or tok >= q1:
+            if tok < q0 or tok >= q1:
                 continue                                      # a row by itself (row_by_warp)
-            assert 0 <= (tok - q0) * group and (tok - q0 + 1) * group <= ROWS
-            unit = s[0] // chunk + b
-            assert 0 <= unit and (s[0] >= ke or (ke - 1) // chunk + b < units)
+            first, n = s[0] // chunk + b, (ke - 1) // chunk - s[0] // chunk + 1 if s[0] < ke else 0
+            by_rows = (q1 - q0) * group > ROWS
+            for row in range((tok - q0) * group, (tok - q0 + 1) * group):
+                if by_rows and n > 0 and row // ROWS >= n:
+                    continue                                  # likewise
+                unit = first + (row // ROWS if by_rows else 0)
+                own = range(unit, unit + (min(n, 1) if by_rows else n))
+                assert all(0 <= u < units for u in own) and (row % ROWS == row or by_rows)
+                if kind == "rising":                          # every result was left, and together they have the row's keys
+                    got = []
+                    for u in own:
+                        assert done[u][0] == b and 0 <= row - done[u][1] < done[u][2]
+                        got += range(max(done[u][3], k_lo), min(done[u][4], k_hi))
+                    assert got == list(range(k_lo, k_hi))
         for t in (0, q_tokens, 2 ** 31 - 1):                  # what the loader may ask for
             keys(at(rng.randrange(seqs)), t)

@@ -54,6 +54,18 @@ def test_own_keys_alone(lens, hq, hk, join_warps, d):
     run(*lens, hq, hk, d, "bf16", 0, None, 0, join_warps, d, causal=False)
 
 
+@pytest.mark.parametrize("d,prefix,parts", [(64, 0, 0), (128, 0, 0), (256, 0, 0), (64, 700, 2)])
+@pytest.mark.parametrize("hq,hk", [(4, 2), (3, 3), (32, 2)])
+@pytest.mark.parametrize("window", [None, 65])
+def test_unused_slots(d, prefix, parts, hq, hk, window):
+    """A batch with unused slots: sequences of many rows, one with more rows than its units take (the rest one by one), one with
+    rows but no keys, between steps of one token."""
+    q_lens = (1, 23, 0, 40, 1, 5, 30) + (0,) * 93
+    k_lens = (500, 1700, 9, 70, 1900, 0, 45) + (0,) * 92 + (3,)
+    run(q_lens, k_lens, hq, hk, d, "bf16", prefix, window, parts, 1, d + hq)
+    run(q_lens, k_lens, hq, hk, d, "fp16", prefix, None, parts, 1, d + hq, causal=False)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("window", [None, 1200])
 @pytest.mark.parametrize("d,prefix", [(64, 0), (128, 0), (256, 0), (64, 300), (64, 2100)])
