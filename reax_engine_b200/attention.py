@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd import forward_ad
@@ -22,11 +23,12 @@ from .moe import _require_cuda
 _DTYPES = {torch.bfloat16: L.BF16, torch.float16: L.FP16}
 
 # What the checks of a call found for one set of shapes, strides, types and options (of tensors that need no copy): the argument
-# block without its pointers and the workspace's size. Emptied when the SM budget changes, on which the size depends.
+# block behind its pointers and the workspace's size. Emptied when the SM budget changes, on which the size depends.
 _checked: dict = {}
-_unused: dict = {}        # device -> the workspace of calls that use none
+_unused: dict = {}        # device number -> the workspace of calls that use none
 _CHECKED_MAX = 4096
-_status: dict = {}        # device -> the status word of calls that are given none
+_status: dict = {}        # device number -> the status word of calls that are given none, and its address
+_POINTERS = struct.Struct("10Q")     # q, k, v, prefix_k, prefix_v, cu_q, cu_k, out, lse, status: the first of AttentionArgs
 _UNUSED = 16             # a workspace of this size is never touched (reaxmoe_attention_workspace_size)
 
 
@@ -40,7 +42,7 @@ def attention_status(device: torch.device | str | int | None = None, clear: bool
     device = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)
     if device.type != "cuda":
         raise ValueError("attention runs on CUDA devices")
-    word = _status.get(device if device.index is not None else torch.device("cuda", torch.cuda.current_device()))
+    word, _ = _status.get(torch.cuda.current_device() if device.index is None else device.index, (None, 0))
     if word is None:
         return 0
     code = int(word)
@@ -49,12 +51,14 @@ def attention_status(device: torch.device | str | int | None = None, clear: bool
     return code
 
 
-def _default_status(device: torch.device) -> torch.Tensor | None:
-    """The device's status word: none before the first call of a process that is not being captured (which could not zero it)."""
-    word = _status.get(device)
-    if word is None and not torch.cuda.is_current_stream_capturing():
-        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
-    return word
+def _default_status(device: torch.device) -> int:
+    """The address of the device's status word: none before the first call of a process that is not being captured (which could
+    not zero it)."""
+    if torch.cuda.is_current_stream_capturing():
+        return 0
+    word = torch.zeros(1, dtype=torch.int32, device=device)
+    _status[device.index] = word, word.data_ptr()
+    return word.data_ptr()
 
 
 def _readable(t: torch.Tensor) -> bool:
@@ -94,7 +98,7 @@ def _output(out: torch.Tensor, q: torch.Tensor, inputs) -> torch.Tensor:
 
 
 def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window):
-    """The argument block of these tensors without its pointers, and the workspace's size."""
+    """The argument block of these tensors behind its pointers, and the workspace's size."""
     ts = [("q", q), ("k", k), ("v", v)] + ([] if prefix_k is None else [("prefix_k", prefix_k), ("prefix_v", prefix_v)])
     if q.dtype not in _DTYPES:
         raise ValueError(f"q must be bf16 or fp16, not {q.dtype}")
@@ -120,13 +124,14 @@ def _check(q, k, v, prefix_k, prefix_v, seqs, seqs_k, dst, scale, causal, window
     need = L.lib().reaxmoe_attention_workspace_size(ctypes.byref(args))
     if need == 0:
         raise L.ReaxMoEError(L.ERR_BAD_SHAPE, L.last_error())
-    return bytes(args), need
+    return bytes(args)[_POINTERS.size:], need
 
 
 def _no_gradients(ts) -> None:
-    for t in ts:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise ValueError("this attention has no backward: detach its inputs or call it under torch.no_grad()")
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise ValueError("this attention has no forward-mode derivative: unpack its inputs")
 
@@ -145,7 +150,10 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         with torch.cuda.device(device):
             return _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, causal, window, return_lse, out,
                               workspace, status)
-    _no_gradients((q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v))
+    index = device.index
+    ts = (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v)
+    if q.requires_grad or k.requires_grad or v.requires_grad or prefix_k is not None or forward_ad._current_level >= 0:
+        _no_gradients(ts)
     cu_q = _lengths(cu_seqlens, "cu_seqlens", device)
     cu_k = cu_q if cu_seqlens_k is None else _lengths(cu_seqlens_k, "cu_seqlens_k", device)
     shape = q.shape
@@ -154,13 +162,14 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
             raise ValueError("q must be [tokens, heads, head_dim]")
         dst = torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=q.dtype, device=device)
     else:
-        dst = _output(out, q, (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v))
+        dst = _output(out, q, ts)
     if status is None:
-        status = _status.get(device)
-        if status is None:
-            status = _default_status(device)
+        found = _status.get(index)
+        status_at = _default_status(device) if found is None else found[1]
     elif status.dtype != torch.int32 or status.device != device or status.numel() < 1:
         raise ValueError("status must be an int32 tensor on the device of q")
+    else:
+        status_at = status.data_ptr()
     if scale is not None:
         scale = float(scale)
     if window is not None:
@@ -175,11 +184,11 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         aligned = aligned and _aligned(prefix_k) and _aligned(prefix_v)
     found = _checked.get(key) if aligned else None
     if found is None:
-        for t in (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v):
+        for t in ts:
             _require_cuda(t)
             if t.ndim != 3:
                 raise ValueError("q, k, v and the prefix must be [tokens, heads, head_dim]")
-        as_they_are = all(map(_readable, (q, k, v) if prefix_k is None else (q, k, v, prefix_k, prefix_v)))
+        as_they_are = all(map(_readable, ts))
         q, k, v = _heads(q), _heads(k), _heads(v)
         if prefix_k is not None:
             prefix_k, prefix_v = _heads(prefix_k), _heads(prefix_v)
@@ -192,9 +201,9 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
     lse = torch.empty_strided(shape[:2], (shape[1], 1), dtype=torch.float32, device=device) if return_lse else None
     if workspace is None:
         if need <= _UNUSED:
-            workspace = _unused.get(device)
+            workspace = _unused.get(index)
             if workspace is None:
-                workspace = _unused[device] = torch.empty(_UNUSED, dtype=torch.uint8, device=device)
+                workspace = _unused[index] = torch.empty(_UNUSED, dtype=torch.uint8, device=device)
         else:
             # of this call alone: ordered with the stream, and private to a graph that is being captured
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
@@ -203,16 +212,11 @@ def _attention(q, k, v, prefix_k, prefix_v, cu_seqlens, cu_seqlens_k, scale, cau
         if workspace.device != device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous and on the device of q")
         nbytes = workspace.numel() * workspace.element_size()
-    args = L.AttentionArgs.from_buffer_copy(block)
-    args.q, args.k, args.v, args.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), dst.data_ptr()
-    args.cu_q, args.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
-    if prefix_k is not None:
-        args.prefix_k, args.prefix_v = prefix_k.data_ptr(), prefix_v.data_ptr()
-    if lse is not None:
-        args.lse = lse.data_ptr()
-    if status is not None:
-        args.status = status.data_ptr()
-    rc = L.lib().reaxmoe_attention(ctypes.byref(args), workspace.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device.index))
+    args = L.AttentionArgs.from_buffer_copy(_POINTERS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if prefix_k is None else prefix_k.data_ptr(),
+        0 if prefix_k is None else prefix_v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), dst.data_ptr(),
+        0 if lse is None else lse.data_ptr(), status_at) + block)
+    rc = L.lib().reaxmoe_attention(ctypes.byref(args), workspace.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         L.check(rc)
     if out is None:
