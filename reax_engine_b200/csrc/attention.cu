@@ -881,14 +881,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
       float x0, x1;
       x2_unpack(check, x0, x1);
       uint32_t again = __ballot_sync(0xffffffffu, live && inv == inv && !(x0 + x1 == 0.0f));
+      auto alive = [&]() {                       // the other warps of both CTAs may have to wait for this one
+        if (lane < 2) st_cluster_u32(map_to_rank(smem_u32(const_cast<uint32_t*>(beat)), (uint32_t)lane), (uint32_t)globaltimer());
+      };
+      if (again != 0u) again = unexplained_rows<D, BF>(p.a, again, tok, head, alive);
 #pragma unroll 1
-      while (again != 0u) {
+      for (; again != 0u; again &= again - 1u) {
         const int src = __ffs(again) - 1;
-        again &= again - 1u;
-        // (the other warps of both CTAs may have to wait for this one meanwhile)
-        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src), false, [&]() {
-          if (lane < 2) st_cluster_u32(map_to_rank(smem_u32(const_cast<uint32_t*>(beat)), (uint32_t)lane), (uint32_t)globaltimer());
-        });
+        row_by_warp<D, BF>(p.a, __shfl_sync(0xffffffffu, tok, src), __shfl_sync(0xffffffffu, head, src), false, alive);
       }
     }
   }
