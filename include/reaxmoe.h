@@ -121,7 +121,8 @@ int reaxmoe_forward_prequant(const reaxmoe_forward_args* args, const void* a_sca
 int reaxmoe_route(const float* logits, const float* per_expert_scale, int32_t tokens, int32_t experts,
                   int32_t topk, int32_t* topk_ids, float* topk_weights, void* stream);
 
-/* Caps the grid of this library's persistent kernels (grouped GEMMs, router, combine) at `sms` CTAs, leaving the
+/* Caps the grid of this library's persistent kernels (grouped GEMMs, router, combine, attention: at least a pair of CTAs there,
+ * and without the short kernels that join its partial results) at `sms` CTAs, leaving the
  * other SMs free for kernels that run beside them -- e.g. the NCCL all-to-alls of an overlapped expert-parallel
  * exchange. 0 (the default) = every SM of the device. Process-wide; set it between calls, not during one. */
 void reaxmoe_set_sm_budget(int32_t sms);

@@ -518,6 +518,7 @@ int reaxmoe_attention(const reaxmoe_attention_args* args, void* workspace, size_
   memset(&l, 0, sizeof(l));
   l.a = a;
   l.num_sms = num_sms();
+  l.whole_device = g_sm_budget <= 0 || l.num_sms < g_sm_budget;
   l.timeout_ns = device_timeout_ns();
   l.workspace = workspace;
   const size_t need = attention_workspace(a, l.num_sms);

@@ -1052,7 +1052,7 @@ static int launch_few(const AttentionLaunch& l, const Plan& pl, const Params* pr
   static std::atomic<uint64_t> allowed{0};
   if (allow_smem(few_kernel<D, BF>, FewLayout<D>::total, allowed)) return REAXMOE_ERR_CUDA;
   const int64_t tasks = (int64_t)pl.units * a.kv_heads;
-  const int64_t blocks = (int64_t)l.num_sms * FewLayout<D>::BLOCKS;
+  const int64_t blocks = (int64_t)l.num_sms * (l.whole_device ? FewLayout<D>::BLOCKS : 1);
   const int grid = (int)(tasks < blocks ? tasks : blocks);
   few_kernel<D, BF><<<grid, FEW_WARPS * 32, FewLayout<D>::total, s>>>(f);
   // partial results a row on the average: a warp joins up to about 32

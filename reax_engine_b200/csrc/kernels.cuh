@@ -152,7 +152,8 @@ struct AttentionLaunch {
   reaxmoe_attention_args a;
   void* workspace;
   unsigned long long timeout_ns;
-  int num_sms;
+  int num_sms;         // the persistent grids' upper bound
+  bool whole_device;   // no SM budget: an SM may hold several blocks
 };
 size_t attention_workspace(const reaxmoe_attention_args& a, int num_sms);
 int launch_attention(const AttentionLaunch& l, cudaStream_t s);

@@ -140,3 +140,41 @@ def test_one_infinity_does_not_take_the_prompt_with_it():
     bad = ~torch.isfinite(o)
     assert bad[n // 2:, :, 5].all() and int(bad.sum()) == (n - n // 2) * 32
     assert times[1] < 30 * times[0], times
+
+
+def launches(f):
+    """Names and grids of the kernels that f launches, from a captured graph."""
+    from cuda.bindings import driver
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        f()
+    ok = lambda r: r[1:] if int(r[0]) == 0 else pytest.fail(str(r[0]))  # noqa: E731
+    g = driver.CUgraph(graph.raw_cuda_graph())
+    nodes = ok(driver.cuGraphGetNodes(g, ok(driver.cuGraphGetNodes(g))[1]))[0]
+    found = []
+    for n in nodes:
+        if ok(driver.cuGraphNodeGetType(n))[0] == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            p = ok(driver.cuGraphKernelNodeGetParams(n))[0]
+            name = ok(driver.cuFuncGetName(p.func))[0] if int(p.func) else ok(driver.cuKernelGetName(p.kern))[0]
+            found.append((name.decode(), p.gridDimX))
+    return found
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_grids_within_the_sm_budget(d):
+    import reax_engine_b200 as R
+    q, k, v, pk, pv = tensors(200, 40000, 4, 4, d, "bf16", 1, prefix=700)
+    step = (dev(list(range(201))), dev([200 * i for i in range(201)]))
+    calls = {"step": lambda: R.prompt_attention(q, k, v, *step),
+             "step behind a prefix": lambda: R.shared_prefix_attention(q, k, v, pk, pv, *step),
+             "prompt": lambda: R.prompt_attention(q, k[:200], v[:200], dev_c)}
+    dev_c = dev([0, 200])
+    try:
+        for budget in (0, 20, 7):
+            R.set_sm_budget(budget)
+            for name, f in calls.items():
+                f()
+                grids = [n for k_, n in launches(f) if "pair_kernel" in k_ or "few_kernel" in k_]
+                assert grids and all(n <= (budget or 2 * 148) for n in grids), (name, budget, grids)
+    finally:
+        R.set_sm_budget(0)
