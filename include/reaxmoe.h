@@ -175,11 +175,13 @@ int reaxmoe_gelu_tanh_mul(const void* gate_up, int64_t rows, int32_t inter, void
  * keys) and sees keys j of it with
  *     j <= t (causal) or every j;   j > t - window when window > 0.
  * out[row] = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max), s_j = scale * q . k_j over the keys seen (bf16 / fp16
- * products, fp32 sums; the weights exp(s_j - max) enter the second product rounded to the operands' type), and lse[row] =
- * max + log(sum). A row that sees no key gets out 0 and lse -inf. Keys that a row does not see do not change it, whatever
- * their values (infinities and NaN included); an element with an infinity or NaN among the values that it does see is one
- * of the two. Query head h reads KV head h / (q_heads / kv_heads). Rows of q at and behind
- * cu_q[seqs] are not written. Inference only: there is no backward. */
+ * products, fp32 sums; the weights exp(s_j - max) enter the second product rounded to the operands' type, in fp16 with a
+ * range down to 2^-29, and the divisor as they are), and lse[row] = max + log(sum). A row that sees no key gets out 0 and
+ * lse -inf. Keys that a row does not see do not change it, whatever their values (infinities and NaN included, but such a
+ * value beside the keys of a row costs doing the row again); an element with an infinity or NaN among the values that it
+ * does see is one of the two. Query head h reads KV head h / (q_heads / kv_heads). Rows of q at and behind cu_q[seqs] are
+ * not written. Lengths that do not rise from 0 give undefined values, but no access outside the tensors.
+ * Inference only: there is no backward. */
 enum { REAXMOE_BF16 = 0, REAXMOE_FP16 = 1 };
 
 typedef struct reaxmoe_attention_args {
@@ -205,7 +207,10 @@ typedef struct reaxmoe_attention_args {
 } reaxmoe_attention_args;
 
 /* Bytes of workspace reaxmoe_attention needs for these sizes (0 on bad sizes; 16: none is touched, any 16 bytes will do). It
- * depends on the sizes and the SM budget alone, not on the cumulative lengths. One call at a time may use a workspace. */
+ * depends on the sizes and the SM budget alone, not on the cumulative lengths. One call at a time may use a workspace.
+ * A generation step (q_tokens <= seqs) has 16 rows of partial results for each sequence and chunk of keys, since any sequence
+ * may have several of the rows: 102 MB for 64 sequences of 2304 keys (1.2 GB of keys and values; 16 / 8 heads of 256), 639 MB
+ * for 4096 of them (77 GB), at worst (16 keys a sequence) a quarter more than the keys and values. */
 size_t reaxmoe_attention_workspace_size(const reaxmoe_attention_args* args);
 int reaxmoe_attention(const reaxmoe_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -18,6 +18,11 @@
 //   S = Q K^T          [256 x 128], Q and K from shared memory (128-byte swizzle, K-major);
 //   P = exp2(c S - c m) by 8 warps per CTA, packed to 16 bits over the first half of S's own TMEM columns;
 //   O += P V           [256 x D], P from TMEM, V from shared memory as it lies in memory (MN-major).
+// P is rounded to 16 bits because the tensor core takes it in the type of V (in 32 bits it would be two products, of a high and a
+// low part); the sum that divides adds the weights as they are before it. Each weight is so off by half a step at most, the
+// outputs by 2.1e-3 to 2.3e-3 (bf16) and 2.8e-4 (fp16) relative to their norm, where rounding alone makes 1.65e-3 and 2.1e-4. On
+// rows with one large weight the lagging maximum (below) shows: 1.78e-3 on the decision model's heads against 1.41e-3 of a
+// kernel whose largest weight is always 1. Maxima, sums and O are held in 32 bits.
 // S has 2 buffers of 128 columns beside O (D columns) for D = 256, 3 for D <= 128: the tensor core multiplies S(j + 1) (and
 // S(j + 2)) while the softmax of tile j runs, and the next item's first S while this item's O is written out.
 //
@@ -188,8 +193,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
   constexpr int O_COL = L::O_COL;
   // The maximum in use may lag behind by a factor of 2^THR before O is rescaled, which costs a wait for the product before.
   // Weights in bf16 keep their precision at any size, so only the range of the fp32 sums limits the lag. fp16 weights end at
-  // 2^16; they are shifted up by 2^SHIFT, so that weights down to 2^-18 of the one at the maximum in use keep all bits (a lag
-  // of 2^3 at SHIFT 12, which has 2^-26, made rescaling so frequent that D = 64 took 4500 clocks a tile).
+  // 2^16; they are shifted up by 2^SHIFT, so that weights down to 2^-18 of the one at the maximum in use keep all bits, those
+  // below lose some, and those under 2^-29 vanish from the product: at most 2^-12 of a row's weight for up to 2^17 keys (a lag
+  // of 2^3 at SHIFT 12, which has 2^-26 and 2^-37, made rescaling so frequent that D = 64 took 4500 clocks a tile).
   constexpr float THR = BF ? 64.0f : 11.0f;
   constexpr float SHIFT = BF ? 0.0f : 4.0f;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -984,11 +990,14 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   pl.tiles = (int)ceil_div64(rows, 2 * pl.rows);
   const int64_t base = (int64_t)pl.tiles * a.kv_heads;
   const int pairs = num_sms / 2 > 0 ? num_sms / 2 : 1;
-  // A generation step (no more query tokens than sequences, with some keys each) goes to few_kernel: 64 sequences of about 1000
-  // keys take 62 us there against 211 in tiles at D = 64 (16 KV heads), 66 against 103 at D = 128 (8), 120 against 115 at
-  // D = 256 (8; 64 x 100 keys 24 against 28, one of 16000 36 against 40). With a prefix it is a launch more, which pays from
-  // some own keys on: 256 sequences of 64 behind 8000 60 against 81 us (D = 64), 85 against 80 (D = 128; of 300 behind 2000
-  // 101 against 134), at D = 256 not (64 of 500 behind 4000 94 against 73).
+  // A generation step (no more query tokens than sequences, with some keys each) goes to few_kernel: 64 sequences of 2304 keys
+  // take 143 us there against 453 in tiles at D = 64 (16 KV heads), 137 against 217 at D = 128 (8), 250 against 241 at D = 256
+  // (8); one of 100 keys is quicker in tiles (12 to 18 us against 10 to 14). With a prefix it is a launch more, which pays from
+  // some own keys on at D = 64 (256 sequences of 100 behind 16384: 98 us against 138), at D = 128 from more (of 100 140
+  // against 138, of 500 221 against 289), at D = 256 hardly ever (of 500 282 against 284, 64 of 2500 305 against 289).
+  // Over 380 sizes (1 to 256 sequences of 16 to 2500 keys behind 0 to 16384, 1 to 16 KV heads) what the rule picks takes 3.2,
+  // 1.3 and 1.0 % longer on the geometric average than the better of the two at D = 64, 128 and 256 (tiles alone 30, 12 and
+  // 4 %), and 45 % at worst (256 sequences of 16 keys behind 512, D = 64, 2 KV heads: 33 us against 22).
   pl.few = pl.group <= FEW_ROWS && a.q_tokens <= a.seqs && a.k_tokens >= 16 * (int64_t)a.seqs && a.k_tokens > 0 &&
            (a.prefix == 0 || (a.head_dim == 64 && a.k_tokens >= 4096) || (a.head_dim == 128 && a.k_tokens >= 32768));
   const int64_t keys = a.prefix + (pl.few ? 0 : a.k_tokens);
@@ -1001,8 +1010,9 @@ static Plan plan(const reaxmoe_attention_args& a, int num_sms) {
   pl.items = (int)items;
   pl.pairs = (int)(items < pairs ? items : pairs);
   // units of few_kernel, of at least 64 keys: with few sequences one for every warp of the device (each sequence may have one
-  // more than its share), else about five, so that the ends of sequences even out (64 sequences of about 2304 keys, D = 256: 252
-  // us with two a warp, 241 with three, 236 with five, 235 with eight, whose joining costs more at D = 128)
+  // more than its share), else about five, so that the ends of sequences even out (64 sequences of 2304 keys, D = 256: 260 us
+  // with two a warp, 252 with three and four, 250 with five and six, 251 with eight; D = 128: 139, 136, 139, 138, 140, 141;
+  // 200 of 700, D = 256: 252, 240, 240, 234, 246, 233: more than two matters, how many does not)
   const int64_t warps = ceil_div64((int64_t)num_sms * FEW_WARPS, a.kv_heads);       // for each KV head
   int64_t chunk = ceil_div64(a.k_tokens, warps >= 8 * (int64_t)a.seqs ? warps - a.seqs : 5 * warps);
   chunk = chunk < 64 ? 64 : ceil_div64(chunk, 16) * 16;
