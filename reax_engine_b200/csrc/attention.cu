@@ -859,7 +859,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) pair_ker
               check = x2_fma(z, 0ull, check);
               float z0, z1;
               x2_unpack(z, z0, z1);
-              v[y / 16][(y / 2) & 7] = pack2<BF>(z0, z1);
+              v[y / 16][(y / 2) & 7] = pack2<BF>(in_range<BF>(z0), in_range<BF>(z1));
             }
             if (live) {
               if (p.wide_out) {
@@ -955,7 +955,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    acc[i] = none ? 0.0f : acc[i] * inv;
+    acc[i] = none ? 0.0f : in_range<BF>(acc[i] * inv);
     bad |= !(fabsf(acc[i]) < INFINITY);
   }
   uint16_t* out = static_cast<uint16_t*>(p.a.out) + (int64_t)tok * p.a.out_stride + head * p.a.out_head_stride;

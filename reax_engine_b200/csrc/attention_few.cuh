@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
   uint32_t packed[W / 2];
 #pragma unroll
   for (int x = 0; x < W; x += 2) {
-    const float y0 = none ? 0.0f : acc[x] * inv, y1 = none ? 0.0f : acc[x + 1] * inv;
+    const float y0 = none ? 0.0f : in_range<BF>(acc[x] * inv), y1 = none ? 0.0f : in_range<BF>(acc[x + 1] * inv);
     bad |= !(fabsf(y0) < INFINITY) || !(fabsf(y1) < INFINITY);
     packed[x / 2] = pack2<BF>(y0, y1);
   }

@@ -94,6 +94,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// An output before it is rounded. It is an average of values, but weights that were rounded up to 16 bits before the product may
+// lift it by 2^-11: past fp16's largest value (65504), it is that value. (bf16 ends where fp32 does.)
+template <bool BF>
+__device__ __forceinline__ float in_range(float v) {
+  if constexpr (BF) return v;
+  return fabsf(v) < 66000.0f ? fminf(fmaxf(v, -65504.0f), 65504.0f) : v;
+}
+
 // One row by one warp, 32 keys at a time: lane = key for the scores, lane l = elements [l D/32, (l+1) D/32) for the sums. It
 // reads the keys that the row sees and no others, which tiles of keys cannot: there a key that a row does not see has weight
 // 0, and 0 x (an infinity or NaN of its value) is NaN.

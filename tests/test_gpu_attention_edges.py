@@ -178,3 +178,47 @@ def test_grids_within_the_sm_budget(d):
                 assert grids and all(n <= (budget or 2 * 148) for n in grids), (name, budget, grids)
     finally:
         R.set_sm_budget(0)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("q_lens,k_lens,prefix", [((300,), (300,), 0), ((3, 2), (5000, 400), 0), ((1,) * 8, (700,) * 8, 0),
+                                                  ((1, 40), (3, 40), 3000), ((1,) * 8, (700,) * 8, 1500)])
+def test_values_at_the_end_of_fp16(d, q_lens, k_lens, prefix):
+    """An average of values of 65504 is 65504, not infinite, however the weights round (larger and larger scores, so that the
+    maximum in use lags)."""
+    import reax_engine_b200 as R
+    cq, ck = cu(q_lens), cu(k_lens)
+    q, k, v, pk, pv = tensors(cq[-1], ck[-1], 4, 2, d, "fp16", d, prefix=prefix)
+    q, k = q * 0 + 1, (k * 0.02 + torch.linspace(-3, 6, ck[-1], device="cuda")[:, None, None] / d * 8).half()
+    v[:, :, ::2], v[:, :, 1] = 65504, -65504
+    if prefix:
+        pk = pk * 0.02
+        pv[:, :, ::2], pv[:, :, 1] = 65504, -65504
+    kw = dict(scale=1.0, return_lse=True)
+    o, lse = (R.shared_prefix_attention(q, k, v, pk, pv, dev(cq), dev(ck), **kw) if prefix
+              else R.prompt_attention(q, k, v, dev(cq), dev(ck), **kw))
+    check(o, reference(q, k, v, cq, ck, 1.0, prefix_k=pk, prefix_v=pv), lse)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,seqs,n,prefix", [(2, 1, 130, 0), (1, 1, 130, 0), (1, 1, 34, 0), (2, 20, 130, 0), (2, 1, 2000, 0),
+                                                (1, 30, 200, 600)])
+def test_a_rounded_up_weight_does_not_make_a_value_infinite(d, rows, seqs, n, prefix):
+    """A row's last two keys have 2^10 (1 + 0.55 2^-10) times the weight of 16 before them (and the others none), which fp16 rounds
+    up by 0.45 2^-10 where these 16 are in an earlier tile, relative to whose maximum the weights are: the products with 65504
+    then sum to 65532 times the sum of the weights, nearer to infinity than to 65504."""
+    import math
+    import reax_engine_b200 as R
+    q, k, v = (torch.zeros(m, 1, d, dtype=torch.float16, device="cuda") for m in (rows * seqs, n * seqs, n * seqs))
+    pk, pv = (torch.zeros(prefix, 1, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    q[..., 0], k[..., 0], pk[..., 0] = 1, -30, -30
+    for s in range(seqs):
+        e = (s + 1) * n
+        k[e - 18:e - 2, 0, 0], k[e - 2:e, 0, 0] = 0, 1
+    for t in (v, pv):
+        t[..., ::2], t[..., 1] = 65504, -65504
+    cq, ck = [rows * i for i in range(seqs + 1)], [n * i for i in range(seqs + 1)]
+    scale = (10 + math.log2(1 + 0.55 * 2 ** -10)) * math.log(2)
+    o = (R.shared_prefix_attention(q, k, v, pk, pv, dev(cq), dev(ck), scale=scale) if prefix
+         else R.prompt_attention(q, k, v, dev(cq), dev(ck), scale=scale))
+    check(o, reference(q, k, v, cq, ck, scale, prefix_k=pk if prefix else None, prefix_v=pv if prefix else None))
