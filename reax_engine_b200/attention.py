@@ -237,10 +237,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     The mask is aligned to the end of the keys: with m query rows and n keys, row i sees keys j <= n - m + i (``causal``), of
     those the last ``window`` ones; a row that sees none (m > n) gets 0 and lse -inf. Keys that a row does not see do not
-    change it, whatever they hold (but infinities and NaN beside its keys make it slow: it is done again). ``scale`` defaults to d ** -0.5. Returns o like q, written into ``out`` where given
-    (of a storage of its own; rows at and behind cu_seqlens[-1] are left as they were; without ``out`` their values are
-    undefined), and with
-    ``return_lse`` the natural logarithm of the softmax's sum [tokens, heads] fp32 too.
+    change it, whatever they hold (but infinities and NaN beside its keys make it slow: it is done again). ``scale`` defaults
+    to d ** -0.5. Returns o like q, written into ``out`` where given (of a storage of its own; rows at and behind cu_seqlens[-1]
+    are left as they were; without ``out`` their values are undefined), and with ``return_lse`` the natural logarithm of the
+    softmax's sum [tokens, heads] fp32 too.
 
     ``workspace``: a uint8 buffer of at least ``reaxmoe_attention_workspace_size`` bytes, used by one call at a time (default:
     one from torch's allocator for this call). ``status``: an int32 device tensor that receives a device-timeout code if a bounded

@@ -378,7 +378,9 @@ class DecisionModel:
         cu = cu_seqlens.to(device=self.dev, dtype=torch.int32)
         n = token_ids.numel()
         lens = cu[1:] - cu[:-1]
-        max_len, min_len, code = torch.stack([lens.max(), lens.min(), self._status[0]]).tolist()
+        max_len, min_len, first, end, code = torch.stack([lens.max(), lens.min(), cu[0], cu[-1], self._status[0]]).tolist()
+        if min_len < 0 or first != 0 or end != n:
+            raise ValueError(f"cu_seqlens must rise from 0 to the number of tokens, {n}")
         if code:
             self._status.zero_()
             self._raise_status(code)
@@ -396,7 +398,7 @@ class DecisionModel:
         seq = torch.repeat_interleave(torch.arange(lens.numel(), device=self.dev), lens.long(), output_size=n)
         pos = torch.arange(n, device=self.dev) - cu[:-1].long()[seq] + start
         last = (cu[1:] - 1).long()
-        if max_len > 0:
+        if max_len > 0 or some is None:
             x = self.embed[token_ids.to(self.dev).long()] * self.normalizer
             x = self._layers(x, pos, cu, max_len, last, prefix)
         if some is not None:

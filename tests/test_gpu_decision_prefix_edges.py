@@ -91,3 +91,16 @@ def test_a_wait_that_ran_out_is_not_passed_over(monkeypatch):
     assert model.read_status() == 0
     assert torch.equal(model.forward(ids, cu, opts), good)
     assert torch.equal(model.forward(ids, cu, opts, prefix=state), good_prefix)
+
+
+def test_lengths_that_do_not_fit_the_tokens_are_refused():
+    """Tokens behind the last prompt, prompts behind the last token, a start that is not 0, and lengths that fall: positions and
+    rows would be taken from outside the batch."""
+    model, _, tails, state, opts = prefixed()
+    ids, cu = packed(tails)
+    bad = [(torch.cat([ids, ids[:3]]), cu), (ids[:-1], cu), (ids, cu + 1), (ids, cu[[0, 2, 1, 3]]), (ids[:4], cu[:1].repeat(3))]
+    for t, c in bad:
+        for prefix in (None, state):
+            with pytest.raises(ValueError):
+                model.forward(t, c, opts, prefix=prefix)
+    model.forward(ids, cu, opts, prefix=state)
